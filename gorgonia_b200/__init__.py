@@ -5,4 +5,4 @@ sources (csrc/) and a thin host-side mirror of gorgonia's engine interface used 
 tests and the benchmark. Importing it fails if the library has not been built.
 """
 from ._lib import B200Error, lib, LIB_PATH  # noqa: F401
-from .engine import Engine, Tensor  # noqa: F401
+from .engine import BlockTensor, Engine, Tensor  # noqa: F401

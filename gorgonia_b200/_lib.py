@@ -19,7 +19,9 @@ class B200Error(RuntimeError):
 
 
 OK, ERR_INVALID, ERR_OOM, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT, ERR_STATE = range(7)
-F32, F64, BF16 = 0, 1, 2
+F32, F64, BF16, E4M3, E5M2 = 0, 1, 2, 3, 4
+BLOCK_ROW, BLOCK_COL, BLOCK_TILE = 0, 1, 2
+NO_TOKEN, TOP_MAX = -1, 32
 VV, VS, SV = 0, 1, 2
 ENGINE_MANAGED, ENGINE_NO_DEFER, ENGINE_CONV_GATHER, ENGINE_NO_STREAMK, ENGINE_NO_PAIRS = 1, 2, 4, 8, 16
 CONV_SIMT, CONV_DIRECT, CONV_TC_GATHER, CONV_TC_TMA, CONV_TC_WINDOW = 0, 1, 2, 3, 4
@@ -166,6 +168,11 @@ _SIGS = {
     "b200_reduce": (_i, [_vp, _i, _i, _vp, _vp, _i64, _i64, _i64]),
     "b200_reduce_all": (_i, [_vp, _i, _i, _vp, _i64, _vp]),
     "b200_reduce_all_static": (_i, [_vp, _i, _i, _vp, _i64, _vp]),
+    "b200_quantize_blocks": (_i, [_vp, _i, _i, _i, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "b200_gemm_blocks": (_i, [_vp, _i, _i, _i, _i64, _i64, _i64, _vp, _i, _i, _i64, _vp, _vp, _i, _i, _i64, _vp, _vp, _i64,
+                              _P(Epilogue)]),
+    "b200_token_logprobs": (_i, [_vp, _i, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i, _vp, _vp]),
+    "b200_token_logprobs_bwd": (_i, [_vp, _i, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64]),
     "b200_argmax": (_i, [_vp, _i, _vp, _vp, _i64, _i64, _i64]),
     "b200_conv2d_fwd": (_i, [_vp, _i, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _i, _i, _i, _i,
                              _P(Epilogue)]),

@@ -92,12 +92,15 @@ int sync_stream_checked(b200_engine *e) {
   if (e->flags_dirty) {
     // kernels with bounded waits report a wait that ran out through d_flags[2]
     // d_flags[3]: a gather met an index outside its range; a replayed tape cannot say so itself
-    B200_CHECK_CUDA(e, cudaMemcpyAsync(e->h_flags + 2, e->d_flags + 2, 2 * sizeof(int), cudaMemcpyDeviceToHost,
+    // d_flags[4]: a kernel met a token index outside the vocabulary
+    B200_CHECK_CUDA(e, cudaMemcpyAsync(e->h_flags + 2, e->d_flags + 2, 3 * sizeof(int), cudaMemcpyDeviceToHost,
                                        e->stream));
     B200_CHECK_CUDA(e, cudaStreamSynchronize(e->stream));
     e->flags_dirty = false;
-    const bool gather = e->gather_dirty;
+    const bool gather = e->gather_dirty, tokens = e->tokens_dirty && e->h_flags[4] != 0;
     e->gather_dirty = false;
+    e->tokens_dirty = false;
+    if (tokens) cudaMemsetAsync(e->d_flags + 4, 0, sizeof(int), e->stream);
     if (e->h_flags[2] != 0) {
       e->h_flags[2] = 0;
       cudaMemsetAsync(e->d_flags + 2, 0, sizeof(int), e->stream);
@@ -112,6 +115,8 @@ int sync_stream_checked(b200_engine *e) {
       return set_error(e, B200_ERR_INVALID, "a replayed tape holds a gather whose index lies outside its "
                        "range; those rows were not written");
     }
+    if (tokens)
+      return set_error(e, B200_ERR_INVALID, "a target of b200_token_logprobs lies outside the vocabulary");
     return B200_OK;
   }
   B200_CHECK_CUDA(e, cudaStreamSynchronize(e->stream));
@@ -281,6 +286,7 @@ struct b200_tape {
   std::vector<int64_t> pinned;  // derived forms of constants the tape reads (see b200_engine::pins)
   uint64_t arena_epoch = 0;
   bool has_gather = false;
+  bool has_tokens = false;
 };
 
 // Ends the special treatment of blocks released during a recording that produced no tape.
@@ -302,6 +308,7 @@ int b200_tape_begin(b200_engine *e) {
   e->capture_free.clear();
   e->capture_pins.clear();
   e->capture_has_gather = false;
+  e->capture_has_tokens = false;
   e->capture_launch_base = e->launches;
   return B200_OK;
 }
@@ -341,6 +348,7 @@ int b200_tape_end(b200_engine *e, b200_tape **out) {
   }
   t->arena_epoch = e->arena_epoch;
   t->has_gather = e->capture_has_gather;
+  t->has_tokens = e->capture_has_tokens;
   for (auto &kv : e->capture_free) t->held.push_back(kv.second);
   e->capture_free.clear();
   t->pinned.swap(e->capture_pins);
@@ -364,6 +372,7 @@ int b200_tape_launch(b200_engine *e, b200_tape *t) {
   e->launches += t->launches;
   e->flags_dirty = true;
   if (t->has_gather) e->gather_dirty = true;
+  if (t->has_tokens) e->tokens_dirty = true;
   return B200_OK;
 }
 

@@ -83,6 +83,8 @@ struct b200_engine {
   bool capturing = false;   // between b200_tape_begin and b200_tape_end
   bool capture_has_gather = false;  // the recording holds a gather, whose index check replays with it
   bool gather_dirty = false;        // such a tape was replayed since the last synchronising call
+  bool capture_has_tokens = false;  // the recording holds kernels that check token indices (d_flags[4])
+  bool tokens_dirty = false;        // such a kernel was launched or replayed since the last synchronising call
   // A recorded tape keeps the addresses its kernels were launched with, so arena blocks handed
   // back while recording stay allocated: they may serve later requests of the same recording
   // (stream order), and at b200_tape_end they become the tape's until b200_tape_destroy.

@@ -108,6 +108,41 @@ class Tensor:
             self.ptr = None
 
 
+_F8 = {"e4m3": _lib.E4M3, "e5m2": _lib.E5M2}
+_BLOCK = {"row": (_lib.BLOCK_ROW, 1, 128), "col": (_lib.BLOCK_COL, 128, 1), "tile": (_lib.BLOCK_TILE, 128, 128)}
+
+
+class BlockTensor:
+    """A matrix of 8-bit floating-point values (q, a uint8 tensor) with one float32 scale for each block: "row"
+    blocks are 1 x 128, "col" 128 x 1, "tile" 128 x 128. A value stands for itself times its block's scale."""
+
+    def __init__(self, q, scales, format="e4m3", block="row"):
+        if format not in _F8:
+            raise B200Error(_lib.ERR_INVALID, f"BlockTensor: format {format!r} is not one of {sorted(_F8)}")
+        if block not in _BLOCK:
+            raise B200Error(_lib.ERR_INVALID, f"BlockTensor: block {block!r} is not one of {sorted(_BLOCK)}")
+        if len(q.shape) != 2 or q.dtype != np.uint8:
+            raise B200Error(_lib.ERR_INVALID, f"BlockTensor: values are a matrix of uint8, not {q.dtype} {q.shape}")
+        want = self.scale_shape(q.shape, block)
+        if scales.shape != want or scales.dtype != np.float32:
+            raise B200Error(_lib.ERR_INVALID, f"BlockTensor: {block} blocks of a {q.shape} matrix have float32 scales of "
+                                              f"shape {want}, not {scales.dtype} {scales.shape}")
+        self.q, self.scales, self.format, self.block = q, scales, format, block
+
+    @staticmethod
+    def scale_shape(shape, block):
+        _, br, bc = _BLOCK[block]
+        return -(-int(shape[0]) // br), -(-int(shape[1]) // bc)
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    def free(self):
+        self.q.free()
+        self.scales.free()
+
+
 class Engine:
     def __init__(self, device=0, arena_bytes=1 << 30, managed=False, defer=True, conv_gather=False, streamk=True,
                  pairs=True):
@@ -405,6 +440,87 @@ class Engine:
         t = self.empty(u.shape, np.uint16).set(u)
         t.is_bf16 = True
         return t
+
+    # ---- 8-bit matrices with a scale for each block of 128 ---------------------------------------
+    def empty_blocks(self, shape, block="row", format="e4m3"):
+        q = self.empty(shape, np.uint8)
+        return BlockTensor(q, self.empty(BlockTensor.scale_shape(shape, block), np.float32), format, block)
+
+    def QuantizeBlocks(self, x, prealloc):
+        """Rounds x (a float32 or bf16 matrix) to prealloc, a BlockTensor: see b200_quantize_blocks."""
+        if x.shape != prealloc.shape:
+            raise B200Error(_lib.ERR_INVALID, f"QuantizeBlocks: {x.shape} does not fit {prealloc.shape}")
+        rows, cols = x.shape
+        dt = _lib.BF16 if getattr(x, "is_bf16", False) else dtype_code(x.dtype)
+        check(lib.b200_quantize_blocks(self.h, dt, _F8[prealloc.format], _BLOCK[prealloc.block][0], x.ptr, cols, rows,
+                                       cols, prealloc.q.ptr, cols, prealloc.scales.ptr), self.h)
+        return prealloc
+
+    def MatMulBlocks(self, a, b, prealloc, transA=False, transB=False, bias=None, bias_kind="col", act=None, alpha=0.0,
+                     incr=False):
+        """prealloc = op(a) @ op(b) of two BlockTensors, or prealloc += it with incr; prealloc is float32 or bf16, the
+        bias float32. The blocks of both operands have to lie along k: see b200_gemm_blocks."""
+        (ar, ac), (br, bc) = a.shape, b.shape
+        M, K = (ac, ar) if transA else (ar, ac)
+        K2, N = (bc, br) if transB else (br, bc)
+        if K != K2:
+            raise B200Error(_lib.ERR_INVALID, f"MatMulBlocks: inner dimensions differ ({K} vs {K2})")
+        if prealloc.size != M * N:
+            raise B200Error(_lib.ERR_INVALID, "MatMulBlocks: prealloc has the wrong size")
+        if bias is not None and (bias.dtype != np.float32 or bias.size != (N if bias_kind == "col" else M)):
+            raise B200Error(_lib.ERR_INVALID, "MatMulBlocks: the bias does not match the result")
+        ct = _lib.BF16 if getattr(prealloc, "is_bf16", False) else dtype_code(prealloc.dtype)
+        ep = _epilogue(bias, bias_kind, act, alpha, accumulate=incr)
+        check(lib.b200_gemm_blocks(self.h, ct, int(transA), int(transB), M, N, K,
+                                   a.q.ptr, _F8[a.format], _BLOCK[a.block][0], ac, a.scales.ptr,
+                                   b.q.ptr, _F8[b.format], _BLOCK[b.block][0], bc, b.scales.ptr,
+                                   prealloc.ptr, N, C.byref(ep) if ep else None), self.h)
+        return prealloc
+
+    # ---- log probabilities of given tokens ---------------------------------------------------------
+    @staticmethod
+    def _stat_checks(who, x, rows, stats):
+        stat = np.float64 if x.dtype == np.float64 else np.float32
+        for name, t, size in stats:
+            if t is not None and (t.size != size or t.dtype != stat):
+                raise B200Error(_lib.ERR_INVALID, f"{who}: {name} has to hold {size} values of {np.dtype(stat)}, not "
+                                                  f"{t.size} of {t.dtype}")
+
+    def TokenLogProbs(self, x, targets, logp, entropy=None, lse=None, top_logp=None, top_index=None):
+        """The log probabilities logp of the tokens `targets` (int64, -1 for none) under the logits x (rows, vocab) of
+        float32, float64 or bf16; the rows' entropy; the log of their sums of exponentials; and the best
+        top_index.shape[1] alternatives. What is None is left out: see b200_token_logprobs."""
+        rows, vocab = x.shape
+        top = 0 if top_index is None else top_index.size // max(rows, 1)
+        self._stat_checks("TokenLogProbs", x, rows, (("logp", logp, rows), ("entropy", entropy, rows), ("lse", lse, rows),
+                                                     ("top_logp", top_logp, rows * top)))
+        for t, size in ((targets, rows), (top_index, rows * top)):
+            if t is not None and (t.dtype != np.int64 or t.size != size):
+                raise B200Error(_lib.ERR_INVALID, "TokenLogProbs: tokens are int64, one target for each row and as many "
+                                                  "alternatives for each")
+        dt = _lib.BF16 if getattr(x, "is_bf16", False) else dtype_code(x.dtype)
+        p = [None if t is None else t.ptr for t in (targets, logp, entropy, lse, top_logp, top_index)]
+        check(lib.b200_token_logprobs(self.h, dt, x.ptr, vocab, rows, vocab, p[0], p[1], p[2], p[3], top, p[4], p[5]),
+              self.h)
+        return logp
+
+    def TokenLogProbsDiff(self, x, targets, lse, entropy, grad_logp, prealloc, grad_entropy=None):
+        """The gradient of sum(grad_logp * logp) + sum(grad_entropy * entropy) with respect to the logits x, from the
+        lse and entropy that TokenLogProbs wrote; prealloc may be x: see b200_token_logprobs_bwd."""
+        rows, vocab = x.shape
+        self._stat_checks("TokenLogProbsDiff", x, rows, (("lse", lse, rows), ("entropy", entropy, rows),
+                                                         ("grad_logp", grad_logp, rows),
+                                                         ("grad_entropy", grad_entropy, rows)))
+        if targets.dtype != np.int64 or targets.size != rows:
+            raise B200Error(_lib.ERR_INVALID, "TokenLogProbsDiff: targets are int64, one for each row")
+        bf = getattr(x, "is_bf16", False)
+        if prealloc.size != x.size or prealloc.dtype != x.dtype or getattr(prealloc, "is_bf16", False) != bf:
+            raise B200Error(_lib.ERR_INVALID, "TokenLogProbsDiff: prealloc does not match the logits")
+        check(lib.b200_token_logprobs_bwd(self.h, _lib.BF16 if bf else dtype_code(x.dtype), x.ptr, vocab, rows, vocab,
+                                          targets.ptr, lse.ptr, None if entropy is None else entropy.ptr, grad_logp.ptr,
+                                          None if grad_entropy is None else grad_entropy.ptr, prealloc.ptr, vocab),
+              self.h)
+        return prealloc
 
     # ---- softmax / reductions ---------------------------------------------------------------
     @staticmethod

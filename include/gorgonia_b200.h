@@ -42,6 +42,9 @@ enum {
 
 /* ---- dtypes ------------------------------------------------------------------------- */
 enum { B200_F32 = 0, B200_F64 = 1, B200_BF16 = 2 };
+/* 8-bit floating point, for tensors that carry a scale for each block (b200_quantize_blocks): 4 exponent and 3
+ * mantissa bits, largest value 448, no infinities; 5 and 2 bits, largest value 57344 */
+enum { B200_E4M3 = 3, B200_E5M2 = 4 };
 
 /* ---- pointwise op codes ---------------------------------------------------------------
  * Binary ops mirror ʘBinaryOperatorType (operatorPointwise_binary_const.go:29-47) and the
@@ -418,6 +421,71 @@ int b200_argmax(b200_engine *e, int dtype, const void *x, int64_t *y, int64_t ou
  *     The array keeps the last call's contents; each call clears the word that must start at zero. */
 #define B200_REDUCE_ALL_STATIC_MAX_N ((int64_t)1 << 32)
 int b200_reduce_all_static(b200_engine *e, int dtype, int kind, const void *x, int64_t n, void *y);
+
+/* ---- 8-bit matrices with a scale for each block of 128 ------------------------------------------
+ * No counterpart in gorgonia, whose tensors are float32 or float64: half the bytes of bf16, twice its tensor-core
+ * rate. A quantised R x C matrix is R x C bytes (row-major, leading dimension ldq) of B200_E4M3 or
+ * B200_E5M2 values and one float32 scale for each block; a value stands for itself times its block's scale. Blocks
+ * are 1 x 128 (ROW), 128 x 1 (COL) or 128 x 128 (TILE) from the matrix's first row and column on, the last ones cut
+ * off by its edges; `scales` is the dense row-major array of them: (R, ceil(C/128)), (ceil(R/128), C) or
+ * (ceil(R/128), ceil(C/128)).
+ *
+ * b200_quantize_blocks: x (R x C, B200_F32 or B200_BF16, leading dimension ldx) -> q, scales. A block's scale is the
+ *   least power of two, 2^-126 at least, that brings its largest finite magnitude to 448 (57344) or below, and 1 if
+ *   it holds no finite value but zeros; dividing by it is exact, so each value is rounded once (to nearest, ties to
+ *   even). NaN stays NaN; an infinity becomes NaN in E4M3 and stays one in E5M2; neither has a part in the scale.
+ *   q may not overlap x.
+ *
+ * b200_gemm_blocks: C = act(op(A) op(B) + bias), or C + that (epilogue.accumulate, C of B200_F32 only). op(A) is
+ *   M x K, op(B) K x N, transX != 0 as in b200_gemm. The blocks of an operand must lie 128 along k: A is ROW or TILE,
+ *   with transA COL or TILE; B is COL or TILE, with transB ROW or TILE. The scales are any float32 values.
+ *   ctype, C's type: B200_F32 or B200_BF16. Products are summed in fp32 over a block of 128 k on the tensor cores; a block's
+ *   sum times its two scales is added up in fp32 registers, and the epilogue is applied there: one rounding at the
+ *   end. ep->bias is a float32 vector for either ctype. K = 0 is the empty sum. C may not overlap the operands.
+ *   Any alignment and leading dimension: operands that the TMA unit cannot read in place (a base or a leading
+ *   dimension that is no multiple of 16 bytes) are copied to arena scratch first, where the arena has room;
+ *   CUDA cores make the product otherwise. Tiles whose k range is shared between CTAs are summed in a fixed order: the
+ *   same call gives the same bits. B200_ENGINE_NO_STREAMK keeps the order of summation the same whatever M is. */
+enum { B200_BLOCK_ROW = 0, B200_BLOCK_COL = 1, B200_BLOCK_TILE = 2 };
+int b200_quantize_blocks(b200_engine *e, int dtype, int qtype, int block, const void *x, int64_t ldx,
+                         int64_t rows, int64_t cols, void *q, int64_t ldq, float *scales);
+int b200_gemm_blocks(b200_engine *e, int ctype, int transA, int transB, int64_t M, int64_t N, int64_t K,
+                     const void *A, int a_type, int a_block, int64_t lda, const float *a_scales,
+                     const void *B, int b_type, int b_block, int64_t ldb, const float *b_scales,
+                     void *C, int64_t ldc, const b200_epilogue *ep);
+
+/* ---- log probabilities of given tokens -----------------------------------------------------------
+ * What a classifier's or language model's loss, and its sampling, read from the logits: in gorgonia a LogSoftMax
+ * (op_softmax.go:99-128) that is written whole, ByIndices on it (op_by_indices.go:90-97), and more passes for the
+ * rest. Here one pass over x (rows x vocab, leading dimension ldx; B200_F32, B200_F64 or B200_BF16) writes for each row,
+ * in float64 for B200_F64 and in float32 otherwise:
+ *   lse     the log of the sum of the exponentials of the row (may be NULL);
+ *   logp    that of the row's target, x[targets[row]] - lse (NULL with targets == NULL); 0 for a row whose target is B200_NO_TOKEN;
+ *   entropy lse - sum p x, p = exp(x - lse) (may be NULL);
+ *   top_logp, top_index (rows x top, top <= B200_TOP_MAX and <= vocab; NULL with top == 0): the `top` largest logits'
+ *     log probabilities and their indices, in descending order, of equal ones the lowest index first; a NaN counts as
+ *     larger than anything.
+ * A logit of -Inf is a token that cannot be: its probability is 0 and it adds nothing to the entropy. A row of nothing
+ * else has lse and log probabilities of -Inf and entropy 0; a row with a NaN or +Inf has NaN in their places.
+ * A target outside [0, vocab) other than B200_NO_TOKEN: logp is NaN, and the next call that waits for the stream
+ * (b200_sync, b200_memcpy_d2h, ...) returns B200_ERR_INVALID, also after the replay of a tape.
+ *
+ * b200_token_logprobs_bwd: the gradient with respect to the logits of sum grad_logp * logp + sum grad_entropy * entropy,
+ *   dx[v] = grad_logp (delta(v = target) - p[v]) - grad_entropy p[v] (ln p[v] + entropy), from the lse and entropy that the
+ *   forward call wrote. Rows whose target is B200_NO_TOKEN have no grad_logp part. grad_entropy may be NULL (then
+ *   entropy is not read). The alternatives carry no gradient. dx (leading dimension lddx) has x's type and may be x
+ *   itself. A row of nothing but -Inf gets zeros. A row without any gradient (no token or grad_logp 0, and grad_entropy
+ *   0 or NULL) gets zeros whatever it holds; its lse and x need not be valid. p = exp(x - lse) with lse as its type
+ *   holds it: logits beyond 10^5 in float32, a row masked with the type's lowest value throughout among them, lose
+ *   digits there. */
+#define B200_NO_TOKEN ((int64_t)-1)
+#define B200_TOP_MAX 32
+int b200_token_logprobs(b200_engine *e, int dtype, const void *x, int64_t ldx, int64_t rows, int64_t vocab,
+                        const int64_t *targets, void *logp, void *entropy, void *lse, int top, void *top_logp,
+                        int64_t *top_index);
+int b200_token_logprobs_bwd(b200_engine *e, int dtype, const void *x, int64_t ldx, int64_t rows, int64_t vocab,
+                            const int64_t *targets, const void *lse, const void *entropy, const void *grad_logp,
+                            const void *grad_entropy, void *dx, int64_t lddx);
 
 /* ---- convolution, pooling, data movement ------------------------------------------------------
  * Tensors are NCHW, dense.
