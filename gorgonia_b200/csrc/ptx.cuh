@@ -405,5 +405,37 @@ __device__ __forceinline__ uint32_t kblock_x3(uint32_t d_main, uint32_t d_tail, 
   return ready;
 }
 
+// 8-bit operands (kind::f8f6f4): the four 32-deep k-slices of a 128-byte k-block into a fresh accumulator, and ONE
+// commit, on a barrier that says both that the stage has been read and that the accumulator is complete.
+// sa / sb: descriptor steps between k-slices (bytes >> 4).
+__device__ __forceinline__ uint32_t kblock_f8(uint32_t d, uint64_t a, uint64_t b, uint64_t sa, uint64_t sb, uint32_t idesc,
+                                              uint32_t done_bar, uint32_t next_full, uint32_t next_parity) {
+  uint32_t ready;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred pn, p0, p1;\n\t"
+      ".reg .b64 a1, b1;\n\t"
+      "setp.ne.b32 p0, %1, %1;\n\t"
+      "setp.eq.b32 p1, %1, %1;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 pn, [%8], %9;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %2, %3, %6, p0;\n\t"
+      "add.s64 a1, %2, %4;\n\t"
+      "add.s64 b1, %3, %5;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], a1, b1, %6, p1;\n\t"
+      "add.s64 a1, a1, %4;\n\t"
+      "add.s64 b1, b1, %5;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], a1, b1, %6, p1;\n\t"
+      "add.s64 a1, a1, %4;\n\t"
+      "add.s64 b1, b1, %5;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], a1, b1, %6, p1;\n\t"
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t"
+      "selp.u32 %0, 1, 0, pn;\n\t"
+      "}"
+      : "=r"(ready)
+      : "r"(d), "l"(a), "l"(b), "l"(sa), "l"(sb), "r"(idesc), "r"(done_bar), "r"(next_full), "r"(next_parity)
+      : "memory");
+  return ready;
+}
+
 }  // namespace ptx
 }  // namespace b200

@@ -47,7 +47,8 @@ __device__ __forceinline__ uint64_t desc_pack(uint32_t lo, uint32_t hi) {
 
 // Instruction descriptor of kind::f16 / kind::tf32: D format F32 (1) at [4,6), A format [7,10),
 // B format [10,13) (1 = BF16, 2 = TF32), A major [15], B major [16] (1 = MN-major),
-// N >> 3 at [17,23), M >> 4 at [24,29).
+// N >> 3 at [17,23), M >> 4 at [24,29). kind::f8f6f4 has the same fields, with 0 = E4M3 and 1 = E5M2 as formats,
+// which may differ between A and B.
 __host__ __device__ constexpr uint32_t make_idesc(int fmt, int a_mn, int b_mn, int M, int N) {
   return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)a_mn << 15) |
          ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
@@ -158,7 +159,7 @@ inline bool streamk_tail_pays(long long tiles, int num_k, int sm_count, int *fir
 
 // A 3-D tensor map (contiguous dim, rows, batch) over a row-major matrix with `ld` elements per
 // row, 128-byte swizzle (atom32: the 32-byte-atom variant that 32-bit MN-major operands need).
-// es = element size in bytes (2: bfloat16, 4: float32). Defined in gemm_tc.cu.
+// es = element size in bytes (1: 8-bit floating point, 2: bfloat16, 4: float32). Defined in gemm_tc.cu.
 int encode_map(b200_engine *e, CUtensorMap *map, int es, const void *base, long long inner, long long rows,
                long long batch, long long ld, long long batch_stride, int box_inner, int box_rows, bool atom32);
 
