@@ -121,7 +121,8 @@ struct BlocksTcParams {
   int a_shift, b_shift;
   void *C;
   long long c_row, c_col;       // elements between rows and columns; one of them is 1
-  int c_bf16, c_vec;            // c_vec: rows can be stored 16 bytes at a time
+  int c_bf16;
+  int c_vec, c_tma;             // rows can be stored 16 bytes at a time; the tile leaves by TMA stores
   int tiles_m, tiles_n, num_k, group_m;
   int stages, stage_bytes;
   // how the work is shared between the CTAs (TilePieces, tc_common.cuh)
@@ -131,6 +132,11 @@ struct BlocksTcParams {
   Epilogue ep;                  // bias_kind in terms of the tiles' rows and columns
   int *err_flag;
 };
+
+constexpr int gb_epi_warps(int bn) { return bn >= 64 ? 8 : 4; }
+constexpr int gb_max_stages(int bn) { return bn >= 128 ? 6 : 12; }
+constexpr int gb_threads(int bn) { return 128 + 32 * gb_epi_warps(bn); }
+constexpr int GB_OUT = 8192;   // bytes of a warp's buffer for the store: two boxes of 32 rows of 128 bytes
 
 // acc += part * scale for two values at a time: the fp32 units take 64-bit operand pairs, and with one fused
 // multiply-add for each value of each k-block they are as busy as the tensor core.
@@ -146,32 +152,54 @@ __device__ __forceinline__ void fma_pair(float &a0, float &a1, uint32_t p0, uint
       : "+f"(a0), "+f"(a1)
       : "r"(p0), "r"(p1), "f"(s0), "f"(s1));
 }
+// acc += part * (row * col), the scales multiplied first.
+__device__ __forceinline__ void scale_fma_pair(float &a0, float &a1, uint32_t p0, uint32_t p1, float row, float c0, float c1) {
+  asm("{\n\t"
+      ".reg .b64 a, p, s, r;\n\t"
+      "mov.b64 a, {%0, %1};\n\t"
+      "mov.b64 p, {%2, %3};\n\t"
+      "mov.b64 r, {%4, %4};\n\t"
+      "mov.b64 s, {%5, %6};\n\t"
+      "mul.rn.f32x2 s, r, s;\n\t"
+      "fma.rn.f32x2 a, p, s, a;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t"
+      "}"
+      : "+f"(a0), "+f"(a1)
+      : "r"(p0), "r"(p1), "f"(row), "f"(c0), "f"(c1));
+}
 
-// Warps: 0 loads (TMA), 1 issues MMAs and owns tensor memory, the others (8, or 4 where a tile is 32 columns or
-// fewer) take each k-block's accumulator to registers, scaled, and store the tile at its end. A ring stage and an
+// Warps: 0 loads (TMA), 1 issues MMAs and owns tensor memory, 2 and 3 bring the scales of the k-blocks into shared
+// memory, the others (8, or 4 where a tile is 32 columns or fewer) take each k-block's accumulator to registers, scaled, and store the tile at its end. A ring stage and an
 // accumulator are one k-block each; there are at least as many stages as accumulators, so that one commit per
 // k-block, on the stage's "done" barrier, serves the loader and the epilogue: that barrier's next phase cannot
 // complete before the epilogue has let go of the accumulator that this one announced.
-template <int BN>
-__global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
+// PAIR: two CTAs of a cluster share a tile of 256 x 256. Each loads its own 128 rows of A and half of B's, the even one
+// issues the MMAs for both (cta_group::2) and keeps their barriers, each scales and stores its own 128 rows.
+template <int BN, bool PAIR>
+__global__ void __launch_bounds__(gb_threads(BN), 1)
     gemm_blocks_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                          const __grid_constant__ BlocksTcParams p) {
+                          const __grid_constant__ CUtensorMap tmC, const __grid_constant__ BlocksTcParams p) {
   ptx::grid_begin();
-  constexpr int EPI_WARPS = BN >= 64 ? 8 : 4;
+  constexpr int EPI_WARPS = gb_epi_warps(BN);
   constexpr int HALF = BN / (EPI_WARPS / 4);    // columns an epilogue warp takes
   constexpr int NBUF = BN == 256 ? 2 : 4;       // accumulators in tensor memory
-  constexpr int CH = HALF < 32 || HALF == 128 ? 16 : 32;  // columns per tcgen05.ld; 128 sums leave no registers for 32
-  constexpr int MAX_STAGES = 12;
+  constexpr int CH = HALF >= 64 ? 64 : HALF;    // columns of the accumulator in registers at a time
+  constexpr int RANKS = PAIR ? 2 : 1;
+  constexpr int MAX_STAGES = gb_max_stages(BN);
   extern __shared__ __align__(1024) unsigned char gb_smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], done_bar[MAX_STAGES], acc_empty[NBUF];
   __shared__ __align__(8) uint64_t epi_bar;  // the epilogue warps meet here when a partial tile is handed over
-  __shared__ __align__(16) float s_col[EPI_WARPS][2][HALF];
+  constexpr int SLOTS = 8, SLOT = GB_BM + BN;   // a ring of its own: scales of the tile's rows and columns, one slot per k-block
+  __shared__ __align__(16) float s_scale[SLOTS][SLOT];
+  __shared__ __align__(8) uint64_t scale_full[SLOTS], scale_empty[SLOTS];
   __shared__ uint32_t tmem_base_s;
   __shared__ int s_fail, s_last;
 
   unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)gb_smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char *stage_out = smem + (size_t)p.stages * p.stage_bytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int stages = p.stages, worker = (int)blockIdx.x, workers = (int)gridDim.x;
+  const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0u;  // 0: the CTA that issues the pair's MMAs
+  const int stages = p.stages, worker = (int)blockIdx.x / RANKS, workers = (int)gridDim.x / RANKS;
   const int total_tiles = p.tiles_m * p.tiles_n;
 
   if (threadIdx.x == 0) {
@@ -179,15 +207,24 @@ __global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
       ptx::mbar_init(&full_bar[s], 1);
       ptx::mbar_init(&done_bar[s], 1);
     }
-    for (int b = 0; b < NBUF; ++b) ptx::mbar_init(&acc_empty[b], EPI_WARPS);
+    for (int b = 0; b < NBUF; ++b) ptx::mbar_init(&acc_empty[b], EPI_WARPS * RANKS);
+    for (int b = 0; b < SLOTS; ++b) {
+      ptx::mbar_init(&scale_full[b], 64);
+      ptx::mbar_init(&scale_empty[b], EPI_WARPS);
+    }
     ptx::mbar_init(&epi_bar, EPI_WARPS);
     ptx::fence_mbar_init();
     s_fail = 0;
     s_last = 0;
   }
   if (warp == 1) {
-    ptx::tmem_alloc(&tmem_base_s, NBUF * BN);
-    ptx::tmem_relinquish();
+    if (PAIR) {
+      ptx::tmem_alloc_pair(&tmem_base_s, NBUF * BN);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(&tmem_base_s, NBUF * BN);
+      ptx::tmem_relinquish();
+    }
   }
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tmap(&tmA);
@@ -195,8 +232,10 @@ __global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
+  if (PAIR) ptx::cluster_sync();  // the other CTA's barriers are initialised before anything reaches them
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = tmem_base_s;
+  auto at_leader = [&](uint64_t *bar) { return ptx::map_to_rank(ptx::smem_addr(bar), 0u); };
 
   // m blocks are walked in groups so that the CTAs of one wave share columns of B and rows of A in L2
   auto decode = [&](int tile, int &mb, int &nb) {
@@ -207,9 +246,12 @@ __global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
     nb = r / gm;
   };
 
-  if (warp == 0) {
+  // 128 sums per thread and what is being added to them need more than an even share of the registers:
+  // 128 x 40 + 256 x 232 = 384 x 168
+  if (warp < 4) {
+    if (BN == 256) ptx::setmaxnreg_dec<40>();
     // ---------------- loads ----------------
-    if (lane == 0) {
+    if (warp == 0 && lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -225,6 +267,22 @@ __global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
           }
           unsigned char *sa = smem + (size_t)stage * p.stage_bytes, *sb = sa + GB_SLAB;
           const int k0 = kb * GB_BK;
+          if (PAIR) {
+            // the even CTA arms the stage for both CTAs' bytes; the odd one's may land first, which only drives the
+            // pending count below zero for a moment
+            if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * (uint32_t)p.stage_bytes);
+            const uint32_t fb = at_leader(&full_bar[stage]);
+            const int m0 = (mb * 2 + (int)rank) * GB_BM, n0 = nb * BN + (int)rank * (BN / 2);
+            if (!p.a_mn) ptx::tma_load_3d_pair(sa, &tmA, k0, m0, 0, fb);
+            else ptx::tma_load_3d_pair(sa, &tmA, m0, k0, 0, fb);
+            if (!p.b_mn) ptx::tma_load_3d_pair(sb, &tmB, k0, n0, 0, fb);
+            else ptx::tma_load_3d_pair(sb, &tmB, n0, k0, 0, fb);
+            if (++stage == stages) {
+              stage = 0;
+              phase ^= 1;
+            }
+            continue;
+          }
           ptx::mbar_arrive_expect_tx(&full_bar[stage], (uint32_t)p.stage_bytes);
           if (!p.a_mn) ptx::tma_load_3d(sa, &tmA, k0, mb * GB_BM, 0, &full_bar[stage]);
           else ptx::tma_load_3d(sa, &tmA, mb * GB_BM, k0, 0, &full_bar[stage]);
@@ -244,51 +302,100 @@ __global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
       }
       if (!ok) s_fail = 1;
     }
-  } else if (warp == 1) {
-    // ---------------- MMAs ----------------
-    if (lane == 0) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, acc_phase = 0;
+    // ---------------- scales ----------------
+    // Rows and columns beyond the matrix get a scale of the last one: they are not stored.
+    if (warp >= 2) {
+      const int t = threadIdx.x - 64;
+      const bool row_each = p.a_shift == 0, col_each = p.b_shift == 0;
+      int slot = 0;
+      uint32_t phase = 0;
       bool ok = true;
-      // a k-slice is 32 bytes of a K-major row, or 32 rows of 128 bytes of an MN-major block
-      const uint64_t a_step = (p.a_mn ? 32 * 128 : 32) >> 4, b_step = (p.b_mn ? 32 * 128 : 32) >> 4;
-      const uint32_t st0 = ptx::smem_addr(smem);
-      const uint64_t a_desc0 = make_smem_desc(st0, p.a_mn ? GB_SLAB : 16, 1024, 2);
-      const uint64_t b_desc0 = make_smem_desc(st0 + GB_SLAB, p.b_mn ? GB_SLAB : 16, 1024, 2);
-      const uint32_t full0 = ptx::smem_addr(&full_bar[0]), done0 = ptx::smem_addr(&done_bar[0]);
-      uint32_t ready = 0;
       TilePieces pieces(p.streamk, p.units, p.num_k, total_tiles, worker, workers, p.sk_first, p.sk_workers);
       int tile, kb0, kb1;
       while (ok && pieces.next(tile, kb0, kb1)) {
+        int mb, nb;
+        decode(tile, mb, nb);
+        const int m0 = (mb * RANKS + (int)rank) * GB_BM, n0 = nb * BN;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!ptx::mbar_wait(&acc_empty[buf], acc_phase ^ 1) || (!ready && !ptx::mbar_wait(&full_bar[stage], phase))) {
+          if (!ptx::mbar_wait_relaxed(&scale_empty[slot], phase ^ 1, 32)) {
             ok = false;
             break;
           }
-          ptx::tc_fence_after_sync();
-          const int ns = stage + 1 == stages ? 0 : stage + 1;
-          const uint32_t nphase = ns == 0 ? phase ^ 1u : phase;
-          const uint64_t soff = (uint64_t)((uint32_t)stage * (uint32_t)(p.stage_bytes >> 4));
-          ready = ptx::kblock_f8(tmem_base + (uint32_t)(buf * BN), a_desc0 + soff, b_desc0 + soff, a_step, b_step, p.idesc,
-                                 done0 + (uint32_t)stage * 8u, full0 + (uint32_t)ns * 8u, nphase);
-          stage = ns;
-          phase = nphase;
-          if (++buf == NBUF) {
-            buf = 0;
-            acc_phase ^= 1;
+          float *to = s_scale[slot];
+          const float *a = p.a_scales + kb * p.as_k, *b = p.b_scales + kb * p.bs_k;
+          if (row_each) {
+#pragma unroll
+            for (int i = 0; i < GB_BM; i += 64) ptx::copy_async_4(to + i + t, a + (long long)min(m0 + i + t, p.M - 1) * p.as_i);
+          } else if (t == 0) {
+            ptx::copy_async_4(to, a + (long long)(min(m0, p.M - 1) >> 7) * p.as_i);
+          }
+          to += GB_BM;
+          if (col_each) {
+#pragma unroll
+            for (int i = 0; i < BN; i += 64)
+              if (i + t < BN) ptx::copy_async_4(to + i + t, b + (long long)min(n0 + i + t, p.N - 1) * p.bs_i);
+          } else if (t * 128 < BN) {
+            ptx::copy_async_4(to + t, b + (long long)(min(n0 + t * 128, p.N - 1) >> 7) * p.bs_i);
+          }
+          ptx::copy_async_arrive(&scale_full[slot]);
+          if (++slot == SLOTS) {
+            slot = 0;
+            phase ^= 1;
           }
         }
+      }
+      ptx::copy_async_wait_all();
+      if (!ok) s_fail = 1;
+    }
+    // ---------------- MMAs (of a pair: the even CTA's only) ----------------
+    if (warp == 1 && rank == 0) {  // all lanes, see kblock_f8
+      // a k-slice is 32 bytes of a K-major row, or 32 rows of 128 bytes of an MN-major block
+      const uint64_t a_step = (p.a_mn ? 32 * 128 : 32) >> 4, b_step = (p.b_mn ? 32 * 128 : 32) >> 4;
+      const uint32_t st0 = ptx::smem_addr(smem), stage_step = (uint32_t)p.stage_bytes >> 4;
+      const uint64_t a_desc0 = make_smem_desc(st0, p.a_mn ? GB_SLAB : 16, 1024, 2);
+      const uint64_t b_desc0 = make_smem_desc(st0 + GB_SLAB, p.b_mn ? GB_SLAB : 16, 1024, 2);
+      const uint32_t done0 = ptx::smem_addr(&done_bar[0]), lead = lane == 0 ? 1u : 0u;
+      // how many k-blocks this CTA takes in all: which tiles they belong to is no concern of this thread
+      int blocks = 0, tile, kb0, kb1;
+      TilePieces pieces(p.streamk, p.units, p.num_k, total_tiles, worker, workers, p.sk_first, p.sk_workers);
+      while (pieces.next(tile, kb0, kb1)) blocks += kb1 - kb0;
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, acc_phase = 1, soff = 0;
+      bool ok = true, full = false, empty = false;  // polled ahead: the next stage is there, the next accumulator is free
+      for (; blocks > 0; --blocks) {
+        if (!__all_sync(0xffffffffu, empty)) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&acc_empty[buf], acc_phase));
+        if (ok && !__all_sync(0xffffffffu, full)) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&full_bar[stage], phase));
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        const uint64_t off = soff;
+        const uint32_t d = tmem_base + (uint32_t)(buf * BN), done = done0 + (uint32_t)stage * 8u;
+        soff += stage_step;
+        if (++stage == stages) {
+          stage = 0;
+          soff = 0;
+          phase ^= 1;
+        }
+        if (++buf == NBUF) {
+          buf = 0;
+          acc_phase ^= 1;
+        }
+        full = ptx::mbar_test_wait(&full_bar[stage], phase);
+        ptx::kblock_f8<PAIR>(lead, d, a_desc0 + off, b_desc0 + off, a_step, b_step, p.idesc, done);
+        empty = ptx::mbar_test_wait(&acc_empty[buf], acc_phase);
       }
       if (!ok) s_fail = 1;
     }
   } else {
+    if (BN == 256) ptx::setmaxnreg_inc<232>();
     // ---------------- scaling, sums and stores ----------------
-    const int ew = warp - 2;
+    const int ew = warp - 4;
     const int quarter = warp & 3;        // the TMEM lanes this warp may read: 32*quarter .. +31
     const int ch0 = (ew >> 2) * HALF;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)ch0;
-    int stage = 0, buf = 0;
-    uint32_t phase = 0, epi_phase = 0;
+    const uint32_t acc_empty0 = at_leader(&acc_empty[0]);
+    int stage = 0, buf = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 0, epi_phase = 0;
+    const bool per_col = p.b_shift == 0;
     bool ok = true;
     auto epi_sync = [&]() -> bool {
       __syncwarp();
@@ -302,77 +409,74 @@ __global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
     while (ok && pieces.next(tile, kb0, kb1)) {
       int mb, nb;
       decode(tile, mb, nb);
-      const int m = mb * GB_BM + quarter * 32 + lane, n0 = nb * BN + ch0;
-      // this thread's row scale, and the warp's column scale(s): one where a tile of scales covers the columns,
-      // else one for each, which the lanes fetch and the warp shares through shared memory. Both are fetched a
-      // k-block ahead. Rows and columns beyond the matrix read a scale of the last one and are not stored.
-      const float *pa = p.a_scales + (long long)(min(m, p.M - 1) >> p.a_shift) * p.as_i;
-      const bool per_col = p.b_shift == 0;
-      const float *pb = p.b_scales + (per_col ? 0 : (long long)(min(n0, p.N - 1) >> 7) * p.bs_i);
-      constexpr int PER = (HALF + 31) / 32;
-      float sa = 0.f, sb = 0.f, sc[PER];
-      auto fetch = [&](int kb) {
-        sa = __ldg(pa + kb * p.as_k);
-        if (per_col) {
-#pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if (j * 32 + lane < HALF) sc[j] = __ldg(p.b_scales + (long long)min(n0 + j * 32 + lane, p.N - 1) * p.bs_i + kb * p.bs_k);
-        } else {
-          sb = __ldg(pb + kb * p.bs_k);
-        }
-      };
+      const int m = (mb * RANKS + (int)rank) * GB_BM + quarter * 32 + lane, n0 = nb * BN + ch0;
+      const int row_at = p.a_shift == 0 ? quarter * 32 + lane : 0, col_at = GB_BM + (per_col ? ch0 : ch0 >> 7);
       float acc[HALF];
 #pragma unroll
       for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
-      if (kb0 < kb1) fetch(kb0);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const float row = sa, both = __fmul_rn(sa, sb);
-        float *cols = s_col[ew][kb & 1];
-        if (per_col) {
+      // An accumulator is taken in pieces of CH columns: the fewer waits for tensor memory, the better (8192^3 with
+      // 16 columns a piece, the next one on its way: 613 us, with 32: 575, with 64 and nothing ahead: 562).
+      uint32_t r[CH];
+      auto load = [&](int c) {
+        const uint32_t at = lane_addr + (uint32_t)(buf * BN + c);
+        if constexpr (CH == 16) {
+          ptx::tmem_ld_32x16(at, r);
+        } else {
 #pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if (j * 32 + lane < HALF) cols[j * 32 + lane] = sc[j];
-          __syncwarp();
+          for (int q = 0; q < CH; q += 32) ptx::tmem_ld_32x32(at + (uint32_t)q, *reinterpret_cast<uint32_t(*)[32]>(&r[q]));
         }
-        if (kb + 1 < kb1) fetch(kb + 1);
-        if (!ptx::mbar_wait(&done_bar[stage], phase)) {
+      };
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!ptx::mbar_wait(&scale_full[slot], slot_phase)) ok = false;  // long there
+        const float *cols = s_scale[slot] + col_at;
+        const float row = s_scale[slot][row_at], both = __fmul_rn(row, *cols);
+        if (!ok || !ptx::mbar_wait(&done_bar[stage], phase)) {
           ok = false;
           break;
+        }
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
         }
         __syncwarp();
         ptx::tc_fence_after_sync();
 #pragma unroll
         for (int c = 0; c < HALF; c += CH) {
-          uint32_t r[CH];
-          if constexpr (CH == 32) ptx::tmem_ld_32x32(lane_addr + (uint32_t)(buf * BN + c), r);
-          else ptx::tmem_ld_32x16(lane_addr + (uint32_t)(buf * BN + c), r);
+          load(c);
           ptx::tmem_ld_wait();
+          if (c + CH == HALF) {
+            ptx::tc_fence_before_sync();  // all of it is in registers: the accumulator is free
+            __syncwarp();
+            if (lane == 0) {
+              if (PAIR) ptx::mbar_arrive_cluster_tmem(acc_empty0 + (uint32_t)buf * 8u);
+              else ptx::mbar_arrive(&acc_empty[buf]);
+            }
+          }
           if (per_col) {
 #pragma unroll
             for (int j = 0; j < CH; j += 4) {
               const float4 s = *reinterpret_cast<const float4 *>(cols + c + j);
-              fma_pair(acc[c + j], acc[c + j + 1], r[j], r[j + 1], __fmul_rn(row, s.x), __fmul_rn(row, s.y));
-              fma_pair(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], __fmul_rn(row, s.z), __fmul_rn(row, s.w));
+              scale_fma_pair(acc[c + j], acc[c + j + 1], r[j], r[j + 1], row, s.x, s.y);
+              scale_fma_pair(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], row, s.z, s.w);
             }
           } else {
 #pragma unroll
             for (int j = 0; j < CH; j += 2) fma_pair(acc[c + j], acc[c + j + 1], r[j], r[j + 1], both, both);
           }
         }
-        ptx::tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&acc_empty[buf]);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
-        }
         if (++buf == NBUF) buf = 0;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&scale_empty[slot]);
+        if (++slot == SLOTS) {
+          slot = 0;
+          slot_phase ^= 1;
+        }
       }
       if (kb0 != 0 || kb1 != p.num_k) {
         // part of a tile: leave it in the workspace; the CTA that delivers the last part finishes the tile
         const int tile_u0 = (tile - p.sk_first) * p.num_k;
-        const size_t slot_floats = (size_t)GB_BM * BN;
-        const size_t within = (size_t)ew * HALF * 32 + lane;
+        const size_t slot_floats = (size_t)GB_BM * BN * RANKS;
+        const size_t within = (size_t)rank * GB_BM * BN + (size_t)ew * HALF * 32 + lane;
         if (ok) {
           float *wsp = p.ws + (size_t)share_slot(worker, tile_u0, p.units, p.sk_workers) * slot_floats + within;
 #pragma unroll
@@ -384,9 +488,10 @@ __global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
         const int c_first = share_of_unit(tile_u0, p.units, p.sk_workers);
         const int c_last = share_of_unit(tile_u0 + p.num_k - 1, p.units, p.sk_workers);
         bool met = epi_sync();
-        if (warp == 2 && lane == 0) {
-          s_last = (atomicAdd(p.tile_count + (tile - p.sk_first), 1) == c_last - c_first) ? 1 : 0;
-          if (s_last) p.tile_count[tile - p.sk_first] = 0;  // zero again for the next launch
+        if (ew == 0 && lane == 0) {  // each CTA of a pair counts for its own rows
+          int *count = p.tile_count + (tile - p.sk_first) * RANKS + (int)rank;
+          s_last = atomicAdd(count, 1) == c_last - c_first ? 1 : 0;
+          if (s_last) *count = 0;  // zero again for the next launch
         }
         met = epi_sync() && met;
         if (!met || *(volatile int *)&s_fail) {
@@ -411,78 +516,146 @@ __global__ void __launch_bounds__(BN >= 64 ? 320 : 192, 1)
           }
         }
       }
-      if (ok && m < p.M && n0 < p.N) {
-        const int valid = min(HALF, p.N - n0);
-        const float *bias = reinterpret_cast<const float *>(p.ep.bias);
-        if (p.ep.bias_kind == B200_BIAS_COL) {
-  #pragma unroll
-          for (int j = 0; j < HALF; ++j)
-            if (j < valid) acc[j] = __fadd_rn(acc[j], __ldg(bias + n0 + j));
-        } else if (p.ep.bias_kind == B200_BIAS_ROW) {
-          const float bm = __ldg(bias + m);
-  #pragma unroll
-          for (int j = 0; j < HALF; ++j) acc[j] = __fadd_rn(acc[j], bm);
+      if (!ok) break;
+      const int mw = m - lane;  // the warp's first row
+      if (mw >= p.M || n0 >= p.N) continue;
+      const int valid = min(HALF, p.N - n0);
+      const float *bias = reinterpret_cast<const float *>(p.ep.bias);
+      if (p.ep.bias_kind == B200_BIAS_COL) {
+#pragma unroll
+        for (int j = 0; j < HALF; ++j)
+          if (j < valid) acc[j] = __fadd_rn(acc[j], __ldg(bias + n0 + j));
+      } else if (p.ep.bias_kind == B200_BIAS_ROW) {
+        const float bm = __ldg(bias + min(m, p.M - 1));
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) acc[j] = __fadd_rn(acc[j], bm);
+      }
+      const float alpha = (float)p.ep.alpha;
+      if (p.ep.act == B200_ACT_RECTIFY) {
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) acc[j] = apply_act<float>(acc[j], B200_ACT_RECTIFY, alpha);
+      } else if (p.ep.act == B200_ACT_LEAKY) {
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) acc[j] = apply_act<float>(acc[j], B200_ACT_LEAKY, alpha);
+      }
+      if (p.c_row == 1) {
+        // swapped: the lanes hold neighbours already
+        if (m < p.M) {
+          const long long at = (long long)n0 * p.c_col + m;
+#pragma unroll
+          for (int j = 0; j < HALF; ++j) {
+            if (j < valid) {
+              const long long x = at + j * p.c_col;
+              if (p.c_bf16) reinterpret_cast<__nv_bfloat16 *>(p.C)[x] = __float2bfloat16_rn(acc[j]);
+              else {
+                float *f = reinterpret_cast<float *>(p.C) + x;
+                *f = p.ep.accumulate ? __fadd_rn(*f, acc[j]) : acc[j];
+              }
+            }
+          }
         }
-        const float alpha = (float)p.ep.alpha;
-        if (p.ep.act == B200_ACT_RECTIFY) {
-  #pragma unroll
-          for (int j = 0; j < HALF; ++j) acc[j] = apply_act<float>(acc[j], B200_ACT_RECTIFY, alpha);
-        } else if (p.ep.act == B200_ACT_LEAKY) {
-  #pragma unroll
-          for (int j = 0; j < HALF; ++j) acc[j] = apply_act<float>(acc[j], B200_ACT_LEAKY, alpha);
-        }
-        const long long at = (long long)m * p.c_row + (long long)n0 * p.c_col;
-        if (p.c_bf16) {
-          __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(p.C) + at;
-          if (p.c_vec && valid == HALF) {
-  #pragma unroll
+      } else {
+        const long long at = (long long)m * p.c_row + n0;
+        if (HALF >= 32 && p.c_tma) {
+          // A lane holds a row. The warp's part of the tile goes to shared memory, boxes of 32 rows of 128 bytes in the
+          // 128-byte swizzle, and from there by TMA stores that drain while the next tile is multiplied: all SMs
+          // come to the end of their tiles together, and stores that were waited for held the accumulators up.
+          const int per = p.c_bf16 ? 64 : 32;
+          unsigned char *out = stage_out + ew * GB_OUT;
+          const int sw = lane & 7;
+          auto send = [&](int c, int boxes) {  // columns c .. of the warp's, in boxes from `out` on
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              for (int i = 0; i < boxes && c + i * per < valid; ++i)
+                ptx::tma_store_3d(&tmC, out + i * 4096, n0 + c + i * per, mw, 0);
+              ptx::bulk_commit();
+            }
+          };
+          auto reuse = [&]() {  // what was sent before has been read
+            if (lane == 0) ptx::bulk_wait_read<0>();
+            __syncwarp();
+          };
+          if (HALF >= 64 && p.c_bf16) {
+            reuse();
+#pragma unroll
             for (int j = 0; j < HALF; j += 8) {
               uint4 w;
               uint32_t *ww = reinterpret_cast<uint32_t *>(&w);
-  #pragma unroll
+#pragma unroll
               for (int t = 0; t < 4; ++t) {
                 const __nv_bfloat162 h = __floats2bfloat162_rn(acc[j + 2 * t], acc[j + 2 * t + 1]);
                 ww[t] = *reinterpret_cast<const uint32_t *>(&h);
               }
-              *reinterpret_cast<uint4 *>(out + j) = w;
+              *reinterpret_cast<uint4 *>(out + (j / 64) * 4096 + lane * 128 + ((((j % 64) / 8) ^ sw) << 4)) = w;
             }
+            send(0, (HALF + 63) / 64);
           } else {
-  #pragma unroll
-            for (int j = 0; j < HALF; ++j)
-              if (j < valid) out[j * p.c_col] = __float2bfloat16_rn(acc[j]);
+#pragma unroll
+            for (int c = 0; c < HALF; c += 64) {
+              reuse();
+#pragma unroll
+              for (int j = c; j < c + 64 && j < HALF; j += 4)
+                *reinterpret_cast<float4 *>(out + ((j - c) / 32) * 4096 + lane * 128 + ((((j % 32) / 4) ^ sw) << 4)) =
+                    make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+              send(c, 2);
+            }
           }
-        } else {
-          float *out = reinterpret_cast<float *>(p.C) + at;
-          if (p.c_vec && valid == HALF) {
-            if (p.ep.accumulate) {  // Incr mode: the rounded result is added to what C holds
-  #pragma unroll
-              for (int j = 0; j < HALF; j += 4) {
-                const float4 old = *reinterpret_cast<const float4 *>(out + j);
-                *reinterpret_cast<float4 *>(out + j) = make_float4(__fadd_rn(old.x, acc[j]), __fadd_rn(old.y, acc[j + 1]),
-                                                                   __fadd_rn(old.z, acc[j + 2]), __fadd_rn(old.w, acc[j + 3]));
+        } else if (m < p.M) {
+          if (p.c_bf16) {
+            __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(p.C) + at;
+            if (p.c_vec && valid == HALF) {
+#pragma unroll
+              for (int j = 0; j < HALF; j += 8) {
+                uint4 w;
+                uint32_t *ww = reinterpret_cast<uint32_t *>(&w);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                  const __nv_bfloat162 h = __floats2bfloat162_rn(acc[j + 2 * t], acc[j + 2 * t + 1]);
+                  ww[t] = *reinterpret_cast<const uint32_t *>(&h);
+                }
+                *reinterpret_cast<uint4 *>(out + j) = w;
               }
             } else {
-  #pragma unroll
-              for (int j = 0; j < HALF; j += 4)
-                *reinterpret_cast<float4 *>(out + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+#pragma unroll
+              for (int j = 0; j < HALF; ++j)
+                if (j < valid) out[j] = __float2bfloat16_rn(acc[j]);
             }
           } else {
-  #pragma unroll
-            for (int j = 0; j < HALF; ++j)
-              if (j < valid) out[j * p.c_col] = p.ep.accumulate ? __fadd_rn(out[j * p.c_col], acc[j]) : acc[j];
+            float *out = reinterpret_cast<float *>(p.C) + at;
+            if (p.c_vec && valid == HALF) {
+#pragma unroll
+              for (int j = 0; j < HALF; j += 4) {
+                float4 v = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                if (p.ep.accumulate) {  // Incr mode: the rounded result is added to what C holds
+                  const float4 old = *reinterpret_cast<const float4 *>(out + j);
+                  v = make_float4(__fadd_rn(old.x, v.x), __fadd_rn(old.y, v.y), __fadd_rn(old.z, v.z), __fadd_rn(old.w, v.w));
+                }
+                *reinterpret_cast<float4 *>(out + j) = v;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < HALF; ++j)
+                if (j < valid) out[j] = p.ep.accumulate ? __fadd_rn(out[j], acc[j]) : acc[j];
+            }
           }
         }
       }
     }
     if (!ok) s_fail = 1;
+    if (lane == 0) ptx::bulk_wait<0>();  // what was sent has been written
   }
 
   ptx::tc_fence_before_sync();
   __syncthreads();
+  // neither CTA of a pair leaves, or gives its tensor memory back, while the other may still read its shared memory
+  // or arrive on its barriers (every wait above is bounded, so both get here)
+  if (PAIR) ptx::cluster_sync();
   if (threadIdx.x == 0 && s_fail) atomicExch(p.err_flag, 1);
   if (warp == 1) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc(tmem_base, NBUF * BN);
+    if (PAIR) ptx::tmem_dealloc_pair(tmem_base, NBUF * BN);
+    else ptx::tmem_dealloc(tmem_base, NBUF * BN);
   }
 }
 
@@ -510,10 +683,11 @@ __global__ void __launch_bounds__(256) repack_kernel(const RepackJob j0, const R
   }
 }
 
-template <int BN>
+// grid: CTAs; pairs launch as clusters of two.
+template <int BN, bool PAIR = false>
 static int launch_blocks_tc(b200_engine *e, const CUtensorMap *tm, const BlocksTcParams &p, int grid) {
-  auto kern = gemm_blocks_tc_kernel<BN>;
-  const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
+  auto kern = gemm_blocks_tc_kernel<BN, PAIR>;
+  const size_t smem = (size_t)p.stages * p.stage_bytes + (p.c_tma ? gb_epi_warps(BN) * GB_OUT : 0) + 1024;
   static std::atomic<int> attr_dev_mask{0};
   if (!(attr_dev_mask & (1 << (e->device & 31)))) {
     cudaFuncAttributes fa;
@@ -522,7 +696,25 @@ static int launch_blocks_tc(b200_engine *e, const CUtensorMap *tm, const BlocksT
     B200_CHECK_CUDA(e, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(optin - fa.sharedSizeBytes)));
     attr_dev_mask |= 1 << (e->device & 31);
   }
-  launch_kernel(e, kern, grid, BN >= 64 ? 320 : 192, smem, tm[0], tm[1], p);
+  if (PAIR) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch_kernel does
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(gb_threads(BN));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = e->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    B200_CHECK_CUDA(e, cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], p));
+  } else {
+    launch_kernel(e, kern, grid, gb_threads(BN), smem, tm[0], tm[1], tm[2], p);
+  }
   B200_CHECK_LAUNCH(e, "gemm_blocks_tc_kernel");
   e->flags_dirty = true;
   return B200_OK;
@@ -574,15 +766,20 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
   int bn = 256;
   while (bn > 64 && (long long)p.tiles_m * ((N + bn - 1) / bn) < e->sm_count) bn /= 2;
   while (bn > 16 && bn / 2 >= N) bn /= 2;
+  p.c_tma = p.c_vec && !ep.accumulate && bn >= (q.c_bf16 ? 128 : 64);  // a warp's columns fill a box of 128 bytes
   p.tiles_n = (int)((N + bn - 1) / bn);
+  // the widest tiles are shared by pairs of CTAs
+  const bool pair = !(e->flags & B200_ENGINE_NO_PAIRS) && bn == 256;
+  if (pair) p.tiles_m = (p.tiles_m + 1) / 2;
+  const int ranks = pair ? 2 : 1, max_workers = e->sm_count / ranks;
   const long long total_tiles = (long long)p.tiles_m * p.tiles_n;
   if (total_tiles >= (1LL << 31))
     return set_error(e, B200_ERR_UNSUPPORTED, "b200_gemm_blocks: %lld output tiles are more than one launch takes", total_tiles);
-  p.group_m = std::min(p.tiles_m, 8);
-  p.stage_bytes = GB_SLAB + (b_mn ? std::max(bn, 128) : bn) * 128;
-  const int budget = (int)std::min<size_t>(e->smem_optin, 227 * 1024) - 1024 - 9 * 1024;  // static part, alignment
-  p.stages = std::min(12, budget / p.stage_bytes);
-  p.idesc = make_idesc(0, a_mn, b_mn, GB_BM, bn) | ((uint32_t)a.e5m2 << 7) | ((uint32_t)b.e5m2 << 10);
+  p.group_m = std::min(p.tiles_m, 8 / ranks);
+  p.stage_bytes = GB_SLAB + (b_mn ? std::max(bn / ranks, 128) : bn / ranks) * 128;
+  const int budget = (int)std::min<size_t>(e->smem_optin, 227 * 1024) - 1024 - 14 * 1024 - (p.c_tma ? gb_epi_warps(bn) * GB_OUT : 0);  // static part, alignment
+  p.stages = std::min(gb_max_stages(bn), budget / p.stage_bytes);
+  p.idesc = make_idesc(0, a_mn, b_mn, GB_BM * ranks, bn) | ((uint32_t)a.e5m2 << 7) | ((uint32_t)b.e5m2 << 10);
 
   // operands that the TMA unit cannot read in place
   void *blk[2] = {nullptr, nullptr};
@@ -608,26 +805,29 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
     if (cudaGetLastError() != cudaSuccess) rc = set_error(e, B200_ERR_CUDA, "launch of repack_kernel failed");
     else e->launches++;
   }
-  CUtensorMap tm[2];
+  CUtensorMap tm[3];
   if (rc == B200_OK) rc = encode_map(e, &tm[0], 1, sa.data, sa.cols, sa.rows, 1, sa.ld, 0, 128, 128, false);
-  if (rc == B200_OK) rc = encode_map(e, &tm[1], 1, sb.data, sb.cols, sb.rows, 1, sb.ld, 0, 128, b_mn ? 128 : bn, false);
-  int grid = (int)std::min<long long>(total_tiles, e->sm_count);
-  p.sk_workers = grid;
+  if (rc == B200_OK) rc = encode_map(e, &tm[1], 1, sb.data, sb.cols, sb.rows, 1, sb.ld, 0, 128, b_mn ? 128 : bn / ranks, false);
+  tm[2] = tm[1];
+  if (rc == B200_OK && p.c_tma)
+    rc = encode_map(e, &tm[2], q.c_bf16 ? 2 : 4, q.C, N, M, 1, q.ldc, 0, q.c_bf16 ? 64 : 32, 32, false);
+  int workers = (int)std::min<long long>(total_tiles, max_workers);
+  p.sk_workers = workers;
   void *ws = nullptr;
   if (rc == B200_OK && !(e->flags & B200_ENGINE_NO_STREAMK)) {
     // whole tiles per CTA would leave SMs idle: share out the k range instead (TilePieces)
-    int sk_grid = grid, first = 0;
-    if (total_tiles <= b200_engine::kSkCounters && streamk_pays(total_tiles, p.num_k, e->sm_count, &sk_grid)) {
-      if (b200_get(e, 2LL * sk_grid * GB_BM * bn * 4, &ws) == B200_OK) {
+    int shares = workers, first = 0;
+    if (total_tiles <= b200_engine::kSkCounters / 2 && streamk_pays(total_tiles, p.num_k, max_workers, &shares)) {
+      if (b200_get(e, 2LL * shares * ranks * GB_BM * bn * 4, &ws) == B200_OK) {
         p.streamk = 1;
         p.units = (int)(total_tiles * p.num_k);
-        grid = p.sk_workers = sk_grid;
+        workers = p.sk_workers = shares;
       }
-    } else if (streamk_tail_pays(total_tiles, p.num_k, e->sm_count, &first, &sk_grid)) {
-      if (b200_get(e, 2LL * sk_grid * GB_BM * bn * 4, &ws) == B200_OK) {
+    } else if (streamk_tail_pays(total_tiles, p.num_k, max_workers, &first, &shares)) {
+      if (b200_get(e, 2LL * shares * ranks * GB_BM * bn * 4, &ws) == B200_OK) {
         p.streamk = 1;
         p.sk_first = first;
-        p.sk_workers = sk_grid;
+        p.sk_workers = shares;
         p.units = (int)((total_tiles - first) * p.num_k);
       }
     }
@@ -636,11 +836,11 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
   }
   if (rc == B200_OK) {
     switch (bn) {
-      case 256: rc = launch_blocks_tc<256>(e, tm, p, grid); break;
-      case 128: rc = launch_blocks_tc<128>(e, tm, p, grid); break;
-      case 64: rc = launch_blocks_tc<64>(e, tm, p, grid); break;
-      case 32: rc = launch_blocks_tc<32>(e, tm, p, grid); break;
-      default: rc = launch_blocks_tc<16>(e, tm, p, grid); break;
+      case 256: rc = pair ? launch_blocks_tc<256, true>(e, tm, p, 2 * workers) : launch_blocks_tc<256>(e, tm, p, workers); break;
+      case 128: rc = launch_blocks_tc<128>(e, tm, p, workers); break;
+      case 64: rc = launch_blocks_tc<64>(e, tm, p, workers); break;
+      case 32: rc = launch_blocks_tc<32>(e, tm, p, workers); break;
+      default: rc = launch_blocks_tc<16>(e, tm, p, workers); break;
     }
   }
   // stream order makes handing the scratch back safe: later users run after this kernel

@@ -62,6 +62,20 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// Whether the phase with the given parity is complete, without waiting.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Waits for the phase with the given parity to complete. Returns false if it did not within
 // `limit_ns` of wall-clock time (default 2 s): the caller then records the failure and leaves.
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint64_t limit_ns = 2000000000ull) {
@@ -97,6 +111,16 @@ __device__ __forceinline__ bool mbar_wait_relaxed(uint64_t *bar, uint32_t parity
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
+
+// ---- small asynchronous copies: four bytes to shared memory, an arrival when the thread's copies so far are there ----
+__device__ __forceinline__ void copy_async_4(void *smem_dst, const void *gmem_src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(smem_dst)), "l"(gmem_src) : "memory");
+}
+// (one of the arrivals that the barrier was initialised for)
+__device__ __forceinline__ void copy_async_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---- bulk copies (no tensor map): 16-byte aligned addresses, size a multiple of 16 -----------
 __device__ __forceinline__ void bulk_g2s(void *smem_dst, const void *gmem_src, uint32_t bytes, uint64_t *bar) {
@@ -134,6 +158,13 @@ __device__ __forceinline__ void tma_load_3d(void *smem_dst, const void *tmap, in
       "[%2];" ::"r"(smem_addr(smem_dst)),
       "l"(tmap), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
+}
+// Store of a box in shared memory (128-byte aligned; the map's swizzle) to a tensor; what lies outside is left out.
+// Part of the thread's bulk group (bulk_commit, bulk_wait).
+__device__ __forceinline__ void tma_store_3d(const void *tmap, const void *smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(tmap),
+               "r"(smem_addr(smem_src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
 }
 // im2col-mode load over an NHWC tensor map (dims C, W, H, N): `pixelsPerColumn` consecutive output
 // positions starting at the window origin (w, h) of image n, walking W, then H, then N inside the
@@ -249,6 +280,12 @@ __device__ __forceinline__ void cluster_sync() {
 // Arrives on an mbarrier given by its shared::cluster address (this CTA's or the other's).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_caddr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_caddr) : "memory");
+}
+// The same where the only thing handed over is tensor memory whose loads tcgen05.wait::ld has seen complete: at CTA
+// scope, without the memory barrier that a release to the cluster makes of it (about a microsecond, once per k-block
+// in the products of 8-bit operands: 8192^3 on pairs 1054 us with it).
+__device__ __forceinline__ void mbar_arrive_cluster_tmem(uint32_t bar_caddr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_caddr) : "memory");
 }
 // Tile-mode load into this CTA's shared memory whose byte count is credited to the mbarrier at
 // `bar_caddr`, which may live in the other CTA of the pair.
@@ -406,35 +443,53 @@ __device__ __forceinline__ uint32_t kblock_x3(uint32_t d_main, uint32_t d_tail, 
 }
 
 // 8-bit operands (kind::f8f6f4): the four 32-deep k-slices of a 128-byte k-block into a fresh accumulator, and ONE
-// commit, on a barrier that says both that the stage has been read and that the accumulator is complete.
-// sa / sb: descriptor steps between k-slices (bytes >> 4).
-__device__ __forceinline__ uint32_t kblock_f8(uint32_t d, uint64_t a, uint64_t b, uint64_t sa, uint64_t sb, uint32_t idesc,
-                                              uint32_t done_bar, uint32_t next_full, uint32_t next_parity) {
-  uint32_t ready;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred pn, p0, p1;\n\t"
-      ".reg .b64 a1, b1;\n\t"
-      "setp.ne.b32 p0, %1, %1;\n\t"
-      "setp.eq.b32 p1, %1, %1;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 pn, [%8], %9;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %2, %3, %6, p0;\n\t"
-      "add.s64 a1, %2, %4;\n\t"
-      "add.s64 b1, %3, %5;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], a1, b1, %6, p1;\n\t"
-      "add.s64 a1, a1, %4;\n\t"
-      "add.s64 b1, b1, %5;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], a1, b1, %6, p1;\n\t"
-      "add.s64 a1, a1, %4;\n\t"
-      "add.s64 b1, b1, %5;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], a1, b1, %6, p1;\n\t"
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t"
-      "selp.u32 %0, 1, 0, pn;\n\t"
-      "}"
-      : "=r"(ready)
-      : "r"(d), "l"(a), "l"(b), "l"(sa), "l"(sb), "r"(idesc), "r"(done_bar), "r"(next_full), "r"(next_parity)
-      : "memory");
-  return ready;
+// commit, on a barrier that says both that the stage has been read and that the accumulator is complete (of a pair:
+// on that barrier of both CTAs). sa / sb: descriptor steps between k-slices (bytes >> 4). The whole warp executes it
+// on values that are the same in all lanes, and the lane whose `lead` is not zero issues: descriptors then stay in
+// uniform registers, where a lone lane moves each through vector registers (about 65 cycles an instruction).
+template <bool PAIR>
+__device__ __forceinline__ void kblock_f8(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint64_t sa, uint64_t sb,
+                                          uint32_t idesc, uint32_t done_bar) {
+#define B200_KB_F8(CG, COMMIT)                                                   \
+  asm volatile(                                                                  \
+      "{\n\t"                                                                    \
+      ".reg .pred pl, p0, p1;\n\t"                                               \
+      ".reg .b64 a1, b1, a2, b2, a3, b3;\n\t"                                    \
+      ".reg .b16 both;\n\t"                                                      \
+      "setp.ne.b32 pl, %0, 0;\n\t"                                               \
+      "setp.ne.b32 p0, %1, %1;\n\t"                                              \
+      "setp.eq.b32 p1, %1, %1;\n\t"                                              \
+      "mov.b16 both, 3;\n\t"                                                     \
+      "add.s64 a1, %2, %4;\n\t"                                                  \
+      "add.s64 b1, %3, %5;\n\t"                                                  \
+      "add.s64 a2, a1, %4;\n\t"                                                  \
+      "add.s64 b2, b1, %5;\n\t"                                                  \
+      "add.s64 a3, a2, %4;\n\t"                                                  \
+      "add.s64 b3, b2, %5;\n\t"                                                  \
+      "@pl tcgen05.mma.cta_group::" CG ".kind::f8f6f4 [%1], %2, %3, %6, p0;\n\t" \
+      "@pl tcgen05.mma.cta_group::" CG ".kind::f8f6f4 [%1], a1, b1, %6, p1;\n\t" \
+      "@pl tcgen05.mma.cta_group::" CG ".kind::f8f6f4 [%1], a2, b2, %6, p1;\n\t" \
+      "@pl tcgen05.mma.cta_group::" CG ".kind::f8f6f4 [%1], a3, b3, %6, p1;\n\t" \
+      "@pl " COMMIT                                                              \
+      "}" ::"r"(lead),                                                           \
+      "r"(d), "l"(a), "l"(b), "l"(sa), "l"(sb), "r"(idesc), "r"(done_bar)        \
+      : "memory")
+  if (PAIR)
+    B200_KB_F8("2", "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%7], both;\n\t");
+  else
+    B200_KB_F8("1", "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t");
+#undef B200_KB_F8
+}
+
+// Moves registers between the warpgroups of a block (all four warps of the warpgroup execute it). The shares must
+// add up to no more than the launch's registers per thread times its threads.
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 }  // namespace ptx

@@ -299,6 +299,24 @@ def test_matmul_repeats_to_the_bit(fresh, M, N, K, ta, tb):
         e.tape_destroy(t)
 
 
+@pytest.mark.parametrize("M,N,K", [(5000, 2048, 300), (4500, 2100, 4096)])
+@pytest.mark.parametrize("ta,tb,bv", [(False, True, False), (False, False, False), (True, False, True)])
+def test_matmul_pairs_of_ctas(fresh, M, N, K, ta, tb, bv):
+    """Large products run on pairs of CTAs, the second with the k ranges of its last tiles shared out: right, and
+    the same bits as on single CTAs where nothing is shared."""
+    e = fresh
+    a, b = operands(19, M, N, K, ta, tb, True, bv)
+    check(multiply(e, a, b, M, N, ta, tb), a, b, K, ta, tb)
+    got = []
+    for pairs in (True, False):
+        one = Engine(0, 256 << 20, streamk=False, pairs=pairs)
+        try:
+            got.append(multiply(one, a, b, M, N, ta, tb))
+        finally:
+            one.Close()
+    assert_bits_equal(got[0], got[1])
+
+
 def test_matmul_order_does_not_depend_on_the_batch():
     """Without shared k ranges a row of the result has the same bits in a batch of any size."""
     e = Engine(0, 256 << 20, streamk=False)
