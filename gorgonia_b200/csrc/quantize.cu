@@ -36,46 +36,241 @@ __device__ __forceinline__ float block_scale(uint32_t amax) {
   return __uint_as_float((uint32_t)max(e, 1) << 23);
 }
 
+// 1 / scale, a power of two from 2^-126 to 2^120.
+__device__ __forceinline__ float inverse(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
+
+// Four values to four bytes; `odd`: an infinity may be among them.
 template <bool E5M2>
-__device__ __forceinline__ uint32_t to_f8(float v) {
-  if (fabsf(v) == INFINITY) return (E5M2 ? 0x7cu : 0x7fu) | (v < 0.f ? 0x80u : 0u);
-  return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
+__device__ __forceinline__ uint32_t to_f8x4(float a, float b, float c, float d, bool odd) {
+  constexpr __nv_fp8_interpretation_t F = E5M2 ? __NV_E5M2 : __NV_E4M3;
+  uint32_t r = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, F) |
+               (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, F) << 16;
+  if (odd) {
+    const float v[4] = {a, b, c, d};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (fabsf(v[j]) == INFINITY) r = (r & ~(0x7fu << (8 * j))) | (E5M2 ? 0x7cu : 0x7fu) << (8 * j);
+  }
+  return r;
 }
 
-// One CTA per block, whatever its shape; two reads of the block.
-template <typename T, bool E5M2>
-__global__ void __launch_bounds__(128) quantize_kernel(const T *__restrict__ x, long long ldx, long long rows, long long cols,
-                                                       uint8_t *__restrict__ q, long long ldq, float *__restrict__ scales,
-                                                       int br, int bc, long long col_blocks) {
+// Values as they are loaded: 16 bytes, or fewer where the rows do not start on 16-byte boundaries (V = 1).
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Values {
+  T v[V];
+};
+
+// V values to V bytes.
+template <typename T, int V, bool E5M2>
+__device__ __forceinline__ void store_f8(uint8_t *q, const Values<T, V> &x, float inv, bool odd) {
+  if constexpr (V == 8) {
+    uint2 w;
+    w.x = to_f8x4<E5M2>(widen<T>(x.v[0]) * inv, widen<T>(x.v[1]) * inv, widen<T>(x.v[2]) * inv, widen<T>(x.v[3]) * inv, odd);
+    w.y = to_f8x4<E5M2>(widen<T>(x.v[4]) * inv, widen<T>(x.v[5]) * inv, widen<T>(x.v[6]) * inv, widen<T>(x.v[7]) * inv, odd);
+    *reinterpret_cast<uint2 *>(q) = w;
+  } else if constexpr (V == 4) {
+    *reinterpret_cast<uint32_t *>(q) =
+        to_f8x4<E5M2>(widen<T>(x.v[0]) * inv, widen<T>(x.v[1]) * inv, widen<T>(x.v[2]) * inv, widen<T>(x.v[3]) * inv, odd);
+  } else {
+    *q = (uint8_t)to_f8x4<E5M2>(widen<T>(x.v[0]) * inv, 0.f, 0.f, 0.f, odd);
+  }
+}
+
+// 1 x 128 blocks: 128 / V lanes hold a block (32 of four values where V = 1), the largest magnitude by shuffles. A
+// warp takes `U` steps of 32 * V consecutive values of a row at a time, all loads first.
+template <typename T, int V, bool E5M2>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T *__restrict__ x, long long ldx, long long rows, long long cols,
+                                                            uint8_t *__restrict__ q, long long ldq, float *__restrict__ scales) {
   ptx::grid_begin();
-  __shared__ uint32_t s_amax;
-  const long long rb = blockIdx.x / col_blocks, cb = blockIdx.x % col_blocks;
-  const int nr = (int)min((long long)br, rows - rb * br), nc = (int)min((long long)bc, cols - cb * bc);
-  x += rb * br * ldx + cb * bc;
-  q += rb * br * ldq + cb * bc;
-  if (threadIdx.x == 0) s_amax = 0;
-  __syncthreads();
-  uint32_t amax = 0;
-  for (int i = threadIdx.x; i < nr * nc; i += blockDim.x) amax = max(amax, finite_magnitude(widen<T>(x[i / nc * ldx + i % nc])));
-  atomicMax(&s_amax, amax);
-  __syncthreads();
-  const float scale = block_scale<E5M2>(s_amax), inv = 1.f / scale;
-  for (int i = threadIdx.x; i < nr * nc; i += blockDim.x)
-    q[i / nc * ldq + i % nc] = (uint8_t)to_f8<E5M2>(widen<T>(x[i / nc * ldx + i % nc]) * inv);
-  if (threadIdx.x == 0) scales[blockIdx.x] = scale;
+  constexpr int U = 4;
+  constexpr int STEP = V == 1 ? 128 : 32 * V;      // values of a row per warp and step
+  constexpr int PER = V == 1 ? 4 : 1;              // loads per lane and step
+  constexpr int LANES = V == 1 ? 32 : 128 / V;     // lanes of a block
+  const int lane = threadIdx.x & 31;
+  const long long blocks = (cols + 127) / 128;
+  for (long long r = blockIdx.y * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8LL) {
+    const T *xr = x + r * ldx;
+    uint8_t *qr = q + r * ldq;
+    for (long long c0 = (long long)blockIdx.x * (U * STEP); c0 < cols; c0 += (long long)gridDim.x * (U * STEP)) {
+      Values<T, V> v[U][PER];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const long long c = c0 + u * STEP + (V == 1 ? i * 32 + lane : lane * V);
+          if (c < cols) {
+            v[u][i] = *reinterpret_cast<const Values<T, V> *>(xr + c);
+          } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[u][i].v[j] = (T)0.f;
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint32_t all = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) all = max(all, __float_as_uint(widen<T>(v[u][i].v[j])) & 0x7fffffffu);
+        uint32_t amax = all;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const bool odd = amax >= 0x7f800000u;
+        if (__any_sync(0xffffffffu, odd)) {  // NaN or infinities: the largest of the others
+          amax = 0;
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) amax = max(amax, finite_magnitude(widen<T>(v[u][i].v[j])));
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        }
+        const float scale = block_scale<E5M2>(amax), inv = inverse(scale);
+        const long long cb = c0 + u * STEP + (V == 1 ? 0 : lane * V);
+        if (lane % LANES == 0 && cb < cols) scales[r * blocks + cb / 128] = scale;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const long long c = c0 + u * STEP + (V == 1 ? i * 32 + lane : lane * V);
+          if (c < cols) store_f8<T, V, E5M2>(qr + c, v[u][i], inv, odd);
+        }
+      }
+    }
+  }
+}
+
+// 128 x 1 blocks (COL) and 128 x 128 ones: a block of 256 threads holds a tile of 128 rows and 16 * V columns (V > 1;
+// 32 columns where V = 1) in registers; columns' maxima are joined through shared memory.
+template <typename T, int V, bool E5M2, bool COL>
+__global__ void __launch_bounds__(256) quantize_tiles_kernel(const T *__restrict__ x, long long ldx, long long rows, long long cols,
+                                                             uint8_t *__restrict__ q, long long ldq, float *__restrict__ scales) {
+  ptx::grid_begin();
+  constexpr int TX = COL ? (V == 1 ? 32 : 16) : (V == 1 ? 32 : 128 / V);  // threads across the columns
+  constexpr int REP = (!COL && V == 1) ? 4 : 1;                           // steps across them
+  constexpr int WIDE = TX * V * REP, TY = 256 / TX, R = 128 / TY;
+  __shared__ uint32_t s_max[COL ? 8 : 1][COL ? WIDE : 8];
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long c0 = (long long)blockIdx.x * WIDE, r0 = (long long)blockIdx.y * 128;
+  Values<T, V> v[R][REP];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int k = 0; k < REP; ++k) {
+      const long long r = r0 + i * TY + ty, c = c0 + (k * TX + tx) * V;
+      if (r < rows && c < cols) {
+        v[i][k] = *reinterpret_cast<const Values<T, V> *>(x + r * ldx + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][k].v[j] = (T)0.f;
+      }
+    }
+  // the largest magnitudes of the block's columns (one value for a tile); finite: without NaN and infinities
+  uint32_t amax[COL ? V : 1];
+  auto largest = [&](bool finite) {
+#pragma unroll
+    for (int j = 0; j < (COL ? V : 1); ++j) amax[j] = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int k = 0; k < REP; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float f = widen<T>(v[i][k].v[j]);
+          uint32_t &m = amax[COL ? j : 0];
+          m = max(m, finite ? finite_magnitude(f) : __float_as_uint(f) & 0x7fffffffu);
+        }
+#pragma unroll
+    for (int o = 16; o >= (COL ? TX : 1); o >>= 1)
+#pragma unroll
+      for (int j = 0; j < (COL ? V : 1); ++j) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
+    __syncthreads();
+    if (COL) {
+      if (lane < TX) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) s_max[warp][tx * V + j] = amax[COL ? j : 0];
+      }
+    } else if (lane == 0) {
+      s_max[0][warp] = amax[0];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < (COL ? V : 1); ++j) {
+      amax[j] = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) amax[j] = max(amax[j], COL ? s_max[w][tx * V + j] : s_max[0][w]);
+    }
+  };
+  largest(false);
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < (COL ? V : 1); ++j) odd |= amax[j] >= 0x7f800000u;
+  if (__syncthreads_or(odd)) largest(true);
+  float inv[COL ? V : 1];
+#pragma unroll
+  for (int j = 0; j < (COL ? V : 1); ++j) {
+    const float scale = block_scale<E5M2>(amax[j]);
+    inv[j] = inverse(scale);
+    if (COL) {
+      if (ty == 0 && c0 + tx * V + j < cols) scales[(long long)blockIdx.y * cols + c0 + tx * V + j] = scale;
+    } else if (threadIdx.x == 0) {
+      scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = scale;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int k = 0; k < REP; ++k) {
+      const long long r = r0 + i * TY + ty, c = c0 + (k * TX + tx) * V;
+      if (r >= rows || c >= cols) continue;
+      uint8_t *to = q + r * ldq + c;
+      if constexpr (COL && V > 1) {
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+          w[j / 4] = to_f8x4<E5M2>(widen<T>(v[i][k].v[j]) * inv[j], widen<T>(v[i][k].v[j + 1]) * inv[j + 1],
+                                   widen<T>(v[i][k].v[j + 2]) * inv[j + 2], widen<T>(v[i][k].v[j + 3]) * inv[j + 3], odd);
+        if constexpr (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t *>(to) = w[0];
+      } else {
+        store_f8<T, V, E5M2>(to, v[i][k], inv[0], odd);
+      }
+    }
+}
+
+template <typename T, int V, bool E5M2>
+static void launch_quantize_as(b200_engine *e, int block, const T *x, long long ldx, long long rows, long long cols, uint8_t *q,
+                               long long ldq, float *scales) {
+  if (block == B200_BLOCK_ROW) {
+    // a warp per row; where rows are few, several per row
+    const long long step = 4 * (V == 1 ? 128 : 32 * V), groups = (rows + 7) / 8, pieces = (cols + step - 1) / step;
+    const long long gx = std::max<long long>(1, std::min(pieces, (16LL * e->sm_count + groups - 1) / groups));
+    launch_kernel(e, quantize_rows_kernel<T, V, E5M2>, dim3((unsigned)gx, (unsigned)std::min<long long>(groups, 65535)), 256, 0, x, ldx,
+                  rows, cols, q, ldq, scales);
+    return;
+  }
+  const bool col = block == B200_BLOCK_COL;
+  const long long wide = col ? (V == 1 ? 32 : 16 * V) : 128;
+  const dim3 grid((unsigned)((cols + wide - 1) / wide), (unsigned)((rows + 127) / 128));
+  if (col) launch_kernel(e, quantize_tiles_kernel<T, V, E5M2, true>, grid, 256, 0, x, ldx, rows, cols, q, ldq, scales);
+  else launch_kernel(e, quantize_tiles_kernel<T, V, E5M2, false>, grid, 256, 0, x, ldx, rows, cols, q, ldq, scales);
 }
 
 template <typename T>
 static int launch_quantize(b200_engine *e, int qtype, int block, const T *x, long long ldx, long long rows, long long cols,
                            uint8_t *q, long long ldq, float *scales) {
-  const int br = block == B200_BLOCK_ROW ? 1 : 128, bc = block == B200_BLOCK_COL ? 1 : 128;
-  const long long rbs = (rows + br - 1) / br, cbs = (cols + bc - 1) / bc;
-  if (rbs * cbs >= (1LL << 31))
-    return set_error(e, B200_ERR_UNSUPPORTED, "b200_quantize_blocks: %lld blocks are more than one launch takes", rbs * cbs);
-  if (qtype == B200_E5M2)
-    launch_kernel(e, quantize_kernel<T, true>, (unsigned)(rbs * cbs), 128, 0, x, ldx, rows, cols, q, ldq, scales, br, bc, cbs);
-  else
-    launch_kernel(e, quantize_kernel<T, false>, (unsigned)(rbs * cbs), 128, 0, x, ldx, rows, cols, q, ldq, scales, br, bc, cbs);
+  constexpr int V = 16 / sizeof(T);
+  if (block != B200_BLOCK_ROW && (rows + 127) / 128 > 65535)
+    return set_error(e, B200_ERR_UNSUPPORTED, "b200_quantize_blocks: %lld rows are more than one launch takes", rows);
+  if ((cols + 31) / 32 >= (1LL << 31))
+    return set_error(e, B200_ERR_UNSUPPORTED, "b200_quantize_blocks: %lld columns are more than one launch takes", cols);
+  // 16-byte loads where every row's vectors lie on their boundaries, and what is stored for them too
+  const bool vec = (uintptr_t)x % 16 == 0 && ldx % V == 0 && (uintptr_t)q % V == 0 && ldq % V == 0 && cols % V == 0;
+  if (qtype == B200_E5M2) {
+    if (vec) launch_quantize_as<T, V, true>(e, block, x, ldx, rows, cols, q, ldq, scales);
+    else launch_quantize_as<T, 1, true>(e, block, x, ldx, rows, cols, q, ldq, scales);
+  } else {
+    if (vec) launch_quantize_as<T, V, false>(e, block, x, ldx, rows, cols, q, ldq, scales);
+    else launch_quantize_as<T, 1, false>(e, block, x, ldx, rows, cols, q, ldq, scales);
+  }
   B200_CHECK_LAUNCH(e, "quantize_kernel");
   return B200_OK;
 }
