@@ -104,6 +104,7 @@ struct Share {
     s += e;
     t = fma(e, fmax(d, Num<S>::far()), t);  // e = 0 for anything as far down, -Inf among it
   }
+  __device__ __forceinline__ void join_lanes();
   __device__ __forceinline__ void join(S m2, S o2, S s2, S t2) {
     if (m2 > m) {
       const S a = m, b = o, c = s, d = t;
@@ -117,6 +118,20 @@ struct Share {
     }
   }
 };
+
+// Every lane's share becomes that of the warp.
+template <typename S>
+__device__ __forceinline__ void Share<S>::join_lanes() {
+  S top = m;
+#pragma unroll
+  for (int o2 = 16; o2 > 0; o2 >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o2));
+  if (top > m) raise(top);
+#pragma unroll
+  for (int o2 = 16; o2 > 0; o2 >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o2);
+    t += __shfl_xor_sync(0xffffffffu, t, o2);
+  }
+}
 
 template <typename T>
 struct LogitTraits { using Stat = float; };
@@ -157,6 +172,7 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
   __shared__ Key b_key[CL > 1 ? B200_TOP_MAX : 1];  // the block's alternatives, in order
   __shared__ uint32_t b_at[CL > 1 ? B200_TOP_MAX : 1];
   __shared__ Share<S> s_share[16], b_share;
+  __shared__ Key b_bound;
   __shared__ uint32_t s_warp[16];
   __shared__ uint32_t s_count;
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
@@ -215,20 +231,51 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
   }
   const S own_max = sh.m;
 
-  // ---- join the sums: lanes, warps, blocks ----
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    sh.join(__shfl_xor_sync(0xffffffffu, sh.m, o), __shfl_xor_sync(0xffffffffu, sh.o, o), __shfl_xor_sync(0xffffffffu, sh.s, o),
-            __shfl_xor_sync(0xffffffffu, sh.t, o));
+  // ---- join the sums: lanes, then warps (by the first one, which finds the bound of the alternatives too) ----
+  const int n = min(a.top, (v1 - v0) * V + (part == 0 ? head : 0) + (part == CL - 1 ? rest : 0));
+  sh.join_lanes();
   if (lane == 0) s_share[warp] = sh;
+  if (n > 0) s_key[tid] = N::key(own_max);
   __syncthreads();
-  sh = s_share[0];
-  for (int w = 1; w < warps; ++w) sh.join(s_share[w].m, s_share[w].o, s_share[w].s, s_share[w].t);
-  if (tid == 0) b_share = sh;
-  const bool wild = sh.s != sh.s;  // of the block's part; the same in every thread
+  if (warp == 0) {
+    sh = lane < warps ? s_share[lane] : Share<S>();
+    sh.join_lanes();
+    if (lane == 0) b_share = sh;
+    if (n > 0) {
+      // the n-th largest of the threads' maxima, bit by bit from the first that they differ in; any bound that n
+      // threads reach will do, so the first one that exactly n reach ends it
+      Key k[16], most = 0, least = ~(Key)0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        k[j] = j < warps ? s_key[j * 32 + lane] : 0;
+        most = max(most, k[j]);
+        if (j < warps) least = min(least, k[j]);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+      }
+      constexpr int BITS = (int)sizeof(Key) * 8;
+      const int same = most == least ? BITS : (BITS == 64 ? __clzll((long long)(most ^ least)) : __clz((int)(most ^ least)));
+      Key bound = same == BITS ? most : most & ~(~(Key)0 >> same);
+      for (int bit = BITS - 1 - same; bit >= 0; --bit) {
+        const Key trial = bound | ((Key)1 << bit);
+        int reach = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) reach += k[j] >= trial ? 1 : 0;
+        reach = __reduce_add_sync(0xffffffffu, reach);
+        if (reach >= n) bound = trial;
+        if (reach == n) break;
+      }
+      if (lane == 0) b_bound = bound;
+    }
+  }
+  __syncthreads();
+  sh = b_share;
+  const bool wild = sh.s != sh.s;  // of the block's part
 
   // ---- the block's alternatives ----
-  const int n = min(a.top, (v1 - v0) * V + (part == 0 ? head : 0) + (part == CL - 1 ? rest : 0));
   // f(value, index) over the share of thread `who`, by the lanes of one warp
   auto scan_share = [&](int who, auto f) {
     if (part == 0 && who < head && lane == 0) f(widen_logit(x[who]), (uint32_t)who);
@@ -261,16 +308,7 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
   if (n > 0) {
     bool search = wild;
     if (!wild) {
-      // the n-th largest of the threads' maxima, bit by bit from the top; any bound that n threads reach will do, so
-      // the first one that exactly n reach ends it
-      const Key mine = N::key(own_max);
-      Key bound = 0;
-      for (int bit = (int)sizeof(Key) * 8 - 1; bit >= 0; --bit) {
-        const Key trial = bound | ((Key)1 << bit);
-        const int reach = __syncthreads_count(mine >= trial);
-        if (reach >= n) bound = trial;
-        if (reach == n) break;
-      }
+      const Key mine = N::key(own_max), bound = b_bound;
       uint32_t who = __ballot_sync(0xffffffffu, mine >= bound);
       while (who) {
         const int l = __ffs((int)who) - 1;
@@ -500,10 +538,10 @@ __global__ void __launch_bounds__(512) token_logprobs_bwd_kernel(const LogprobBw
   for (; i < v1; i += nt) many(i, xv[i]);
 }
 
-// Threads per row: eight vectors each, one warp at least, 512 at most.
+// Threads per row: sixteen vectors each, one warp at least, 512 at most.
 static int row_threads(long long nvec) {
   int nt = 32;
-  while (nt < 512 && nt * 8 < nvec) nt *= 2;
+  while (nt < 512 && nt * 16 < nvec) nt *= 2;
   return nt;
 }
 
