@@ -162,7 +162,7 @@ struct LogprobArgs {
 // One block, or a cluster of CL, per row. V: values per load; a row's head up to the first 16-byte boundary, and its
 // tail, are read one by one.
 template <typename T, int V, int CL>
-__global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T> a) {
+__global__ void __launch_bounds__(CL > 1 ? 512 : 256, CL > 1 ? 2 : 5) token_logprobs_kernel(const LogprobArgs<T> a) {
   ptx::grid_begin();
   using S = typename LogitTraits<T>::Stat;
   using N = Num<S>;
@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
   __shared__ Share<S> s_share[16], b_share;
   __shared__ Key b_bound;
   __shared__ uint32_t s_warp[16];
-  __shared__ uint32_t s_count;
+  __shared__ uint32_t s_count, s_parts;
+  __shared__ uint16_t s_who[512];
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
   const long long row = blockIdx.x / CL;
   const int part = CL > 1 ? (int)(blockIdx.x % CL) : 0;
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
   const int v0 = (int)((long long)nvec * part / CL), v1 = (int)((long long)nvec * (part + 1) / CL);
   const bool has_head = part == 0 && tid < head, has_rest = part == CL - 1 && tid < rest;
   const Pack<T, V> *xv = reinterpret_cast<const Pack<T, V> *>(x + head);
-  if (tid == 0) s_count = 0;
+  if (tid == 0) s_count = s_parts = 0;
 
   S target = 0;
   long long token = B200_NO_TOKEN;
@@ -242,8 +243,8 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
     sh.join_lanes();
     if (lane == 0) b_share = sh;
     if (n > 0) {
-      // the n-th largest of the threads' maxima, bit by bit from the first that they differ in; any bound that n
-      // threads reach will do, so the first one that exactly n reach ends it
+      // towards the n-th largest of the threads' maxima, bit by bit from the first that they differ in, until a bound
+      // is found that n threads reach, and not many more
       Key k[16], most = 0, least = ~(Key)0;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -263,10 +264,11 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
         const Key trial = bound | ((Key)1 << bit);
         int reach = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) reach += k[j] >= trial ? 1 : 0;
+        for (int j = 0; j < 16; j += 4)
+          reach += ((k[j] >= trial) + (k[j + 1] >= trial)) + ((k[j + 2] >= trial) + (k[j + 3] >= trial));
         reach = __reduce_add_sync(0xffffffffu, reach);
         if (reach >= n) bound = trial;
-        if (reach == n) break;
+        if (reach >= n && reach <= 2 * n + 8) break;
       }
       if (lane == 0) b_bound = bound;
     }
@@ -276,15 +278,23 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
   const bool wild = sh.s != sh.s;  // of the block's part
 
   // ---- the block's alternatives ----
-  // f(value, index) over the share of thread `who`, by the lanes of one warp
-  auto scan_share = [&](int who, auto f) {
-    if (part == 0 && who < head && lane == 0) f(widen_logit(x[who]), (uint32_t)who);
-    if (part == CL - 1 && who < rest && lane == 0) f(widen_logit(x[vocab - rest + who]), (uint32_t)(vocab - rest + who));
-    for (int k = v0 + who + lane * nt; k < v1; k += 32 * nt) {
+  // f(value, index) over the shares of the threads whose maximum is above the bound (or at it), by the whole block: one
+  // vector of one share per thread and step. Every thread of the block calls it.
+  const int per = (v1 - v0 + nt - 1) / nt;
+  auto scan_shares = [&](bool takes_part, auto f) {
+    if (takes_part) s_who[atomicAdd(&s_parts, 1u)] = (uint16_t)tid;
+    __syncthreads();
+    const int all = (int)s_parts;
+    for (int c = tid; c < all * per; c += nt) {
+      const int k = v0 + s_who[c / per] + c % per * nt;
+      if (k >= v1) continue;
       const Pack<T, V> b = xv[k];
 #pragma unroll
       for (int j = 0; j < V; ++j) f(widen_logit(b.v[j]), (uint32_t)(head + k * V + j));
     }
+    if (takes_part && has_head) f(widen_logit(x[tid]), (uint32_t)tid);
+    if (takes_part && has_rest) f(widen_logit(x[vocab - rest + tid]), (uint32_t)(vocab - rest + tid));
+    __syncthreads();
   };
   auto push = [&](Key key, uint32_t at) {
     const uint32_t p = atomicAdd(&s_count, 1u);
@@ -309,32 +319,20 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const LogprobArgs<T
     bool search = wild;
     if (!wild) {
       const Key mine = N::key(own_max), bound = b_bound;
-      uint32_t who = __ballot_sync(0xffffffffu, mine >= bound);
-      while (who) {
-        const int l = __ffs((int)who) - 1;
-        who &= who - 1;
-        scan_share(warp * 32 + l, [&](S v, uint32_t at) {
-          const Key k = N::key(v);
-          if (k >= bound) push(k, at);
-        });
-      }
-      __syncthreads();
+      scan_shares(mine >= bound, [&](S v, uint32_t at) {
+        const Key k = N::key(v);
+        if (k >= bound) push(k, at);
+      });
       listed = (int)s_count;
       if (listed > LP_LIST) {
         // many equals: what lies above the bound, then the first equals in the order of the row
         __syncthreads();
-        if (tid == 0) s_count = 0;
+        if (tid == 0) s_count = s_parts = 0;
         __syncthreads();
-        who = __ballot_sync(0xffffffffu, mine > bound);
-        while (who) {
-          const int l = __ffs((int)who) - 1;
-          who &= who - 1;
-          scan_share(warp * 32 + l, [&](S v, uint32_t at) {
-            const Key k = N::key(v);
-            if (k > bound) push(k, at);
-          });
-        }
-        __syncthreads();
+        scan_shares(mine > bound, [&](S v, uint32_t at) {
+          const Key k = N::key(v);
+          if (k > bound) push(k, at);
+        });
         listed = (int)s_count;
         search = listed > LP_LIST;
         int missing = search ? 0 : n - listed;  // the same in every thread, as is what follows
@@ -538,10 +536,10 @@ __global__ void __launch_bounds__(512) token_logprobs_bwd_kernel(const LogprobBw
   for (; i < v1; i += nt) many(i, xv[i]);
 }
 
-// Threads per row: sixteen vectors each, one warp at least, 512 at most.
-static int row_threads(long long nvec) {
+// Threads per row: sixteen vectors each, one warp at least.
+static int row_threads(long long nvec, int most) {
   int nt = 32;
-  while (nt < 512 && nt * 16 < nvec) nt *= 2;
+  while (nt < most && nt * 16 < nvec) nt *= 2;
   return nt;
 }
 
@@ -579,10 +577,13 @@ static int launch_forward(b200_engine *e, const void *x, long long ldx, long lon
     launch_forward_as<T, 1, 1>(e, a, rows, 32);
   } else {
     const long long nvec = vocab / V;
-    const int nt = row_threads(nvec);
-    // few rows are shared by clusters, as long as a block keeps two vectors for each of its threads
-    int cl = 1;
+    // Few rows are shared by clusters, as long as a block keeps two vectors for each of its threads; with as many threads
+    // as a block can have, since nothing else runs on their SMs. Many rows have blocks of 256, five to an SM: what
+    // one of them waits for (its sums' joining, its alternatives) passes behind the others' loads. 4096 x 32000 with
+    // 5 alternatives: blocks of 512 111 us (bf16 83), 256 100 (72), 128 109 (64).
+    int cl = 1, nt = row_threads(nvec, 512);
     while (cl < 8 && rows * cl < e->sm_count && nvec / (2 * cl) >= 2 * nt) cl *= 2;
+    if (cl == 1) nt = row_threads(nvec, 256);
     if (cl == 8) launch_forward_as<T, V, 8>(e, a, rows, nt);
     else if (cl == 4) launch_forward_as<T, V, 4>(e, a, rows, nt);
     else if (cl == 2) launch_forward_as<T, V, 2>(e, a, rows, nt);
@@ -603,7 +604,7 @@ static int launch_backward(b200_engine *e, const void *x, long long ldx, long lo
   // vectors where the rows of x and dx lie alike to 16-byte boundaries
   const bool alike = ((uintptr_t)x - (uintptr_t)dx) % 16 == 0 && (ldx - lddx) * (long long)sizeof(T) % 16 == 0;
   const long long nvec = alike && vocab >= 256 ? vocab / V : vocab;
-  const int nt = row_threads(nvec);
+  const int nt = row_threads(nvec, 512);
   const long long parts = std::max<long long>(1, std::min<long long>((2LL * e->sm_count + rows - 1) / rows, nvec / (4 * nt)));
   if (rows * parts >= (1LL << 31))
     return set_error(e, B200_ERR_UNSUPPORTED, "b200_token_logprobs_bwd: %lld rows are more than one launch takes", rows);
