@@ -105,6 +105,107 @@ __global__ void __launch_bounds__(256) gemm_blocks_simt_kernel(const BlockOperan
 }
 
 // ------------------------------------------------------------------------------------------
+// up to 16 rows of A, both operands with k contiguous: B is read, nothing else counts
+// ------------------------------------------------------------------------------------------
+
+// D += A B for 16 x 8 x 32 8-bit values, in fp32. (tcgen05 has no business here: a tile's way through shared and tensor
+// memory costs more than the reading of B itself. 1 x 4096 x 4096 there: 12.4 us.)
+template <bool A5, bool B5>
+__device__ __forceinline__ void mma_16x8x32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+#define B200_MMA_F8(TA, TB)                                                                                                 \
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32." TA "." TB ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "      \
+               "{%0, %1, %2, %3};"                                                                                         \
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                            \
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+  if (A5 && B5) B200_MMA_F8("e5m2", "e5m2");
+  else if (A5) B200_MMA_F8("e5m2", "e4m3");
+  else if (B5) B200_MMA_F8("e4m3", "e5m2");
+  else B200_MMA_F8("e4m3", "e4m3");
+#undef B200_MMA_F8
+}
+
+// A block takes 16 rows of the weights w and all of x; its eight warps share the k-blocks, and their sums are added in the
+// order of the warps. In a warp, lane 4 g + t holds the 16 bytes from 16 t on of every 64 of rows g and g + 8: which k an
+// instruction's operands belong to does not matter as long as both operands agree. 1 x 4096 x 4096: 6.7 us,
+// of which 2.6 are the reading of B at the copy rate and most of the rest the launch and one way to memory.
+template <int NT, bool W5, bool X5>
+__global__ void __launch_bounds__(256, 2) gemm_blocks_skinny_kernel(const BlockOperand w, const BlockOperand x, const BlocksParams p) {
+  ptx::grid_begin();
+  __shared__ float s_sum[8][16][NT * 8 + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const long long n0 = (long long)blockIdx.x * 16;  // rows of w, columns of C
+  const int nk = (int)((p.K + 127) / 128);
+  const uint8_t *row[2 + NT];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) row[r] = w.data + min(n0 + g + 8 * r, p.N - 1) * w.si;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) row[2 + j] = x.data + min((long long)(j * 8 + g), p.M - 1) * x.si;
+  const float *ws[2], *xs[NT][2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    ws[r] = w.scales + (min(n0 + g + 8 * r, p.N - 1) >> w.shift) * w.ss_i;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) xs[j][r] = x.scales + (min((long long)(j * 8 + 2 * t + r), p.M - 1) >> x.shift) * x.ss_i;
+  }
+  const int K = (int)p.K;  // a multiple of 16
+  auto bytes = [&](int r, int k) -> uint4 {
+    return k < K ? __ldg(reinterpret_cast<const uint4 *>(row[r] + k)) : make_uint4(0, 0, 0, 0);
+  };
+  constexpr int AHEAD = 4;  // k-blocks of w in flight per warp: 2 KB each
+  float acc[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[j][c] = 0.f;
+  for (int kb0 = warp; kb0 < nk; kb0 += 8 * AHEAD) {
+    uint4 v[AHEAD][2][2];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) v[i][h][r] = bytes(r, (kb0 + 8 * i) * 128 + h * 64 + t * 16);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int kb = kb0 + 8 * i;
+      if (kb >= nk) continue;
+      const float sw[2] = {__ldg(ws[0] + kb * w.ss_k), __ldg(ws[1] + kb * w.ss_k)};
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const float sx[2] = {__ldg(xs[j][0] + kb * x.ss_k), __ldg(xs[j][1] + kb * x.ss_k)};
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 &a0 = v[i][h][0], &a1 = v[i][h][1], b = bytes(2 + j, kb * 128 + h * 64 + t * 16);
+          mma_16x8x32<W5, X5>(part, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+          mma_16x8x32<W5, X5>(part, a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[j][c] = __fmaf_rn(part[c], __fmul_rn(sw[c >> 1], sx[c & 1]), acc[j][c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_sum[warp][g + 8 * (i >> 1)][j * 8 + 2 * t + (i & 1)] = acc[j][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * NT * 8; i += 256) {
+    const int r = i & 15, m = i >> 4;
+    const long long n = n0 + r;
+    if (m >= p.M || n >= p.N) continue;
+    float sum = s_sum[0][r][m];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) sum = __fadd_rn(sum, s_sum[q][r][m]);
+    const float out = apply_epilogue<float>(sum, p.ep, m, n);
+    const long long at = m * p.ldc + n;
+    if (p.c_bf16) ((__nv_bfloat16 *)p.C)[at] = __float2bfloat16_rn(out);
+    else ((float *)p.C)[at] = p.ep.accumulate ? __fadd_rn(((float *)p.C)[at], out) : out;
+  }
+}
+
+// ------------------------------------------------------------------------------------------
 // tensor cores
 // ------------------------------------------------------------------------------------------
 
@@ -502,15 +603,27 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
         __threadfence();
 #pragma unroll
         for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
-        for (int c = c_first; c <= c_last; ++c) {  // k order: CTA c's share precedes CTA c + 1's
-          const float *src = p.ws + (size_t)share_slot(c, tile_u0, p.units, p.sk_workers) * slot_floats + within;
-          if constexpr (HALF <= 32) {
-            float part[HALF];
+        // k order: CTA c's share precedes CTA c + 1's. A part is a latency of about a microsecond: on narrow tiles
+        // several are on their way at once
+        constexpr int PF = HALF <= 16 ? 8 : (HALF <= 32 ? 2 : 1);
+        for (int c = c_first; c <= c_last; c += PF) {
+          if constexpr (PF > 1) {
+            float in[PF][HALF];
 #pragma unroll
-            for (int j = 0; j < HALF; ++j) part[j] = __ldcg(src + j * 32);
+            for (int q = 0; q < PF; ++q) {
+              const float *src = p.ws + (size_t)share_slot(min(c + q, c_last), tile_u0, p.units, p.sk_workers) * slot_floats + within;
 #pragma unroll
-            for (int j = 0; j < HALF; ++j) acc[j] = __fadd_rn(acc[j], part[j]);
+              for (int j = 0; j < HALF; ++j) in[q][j] = __ldcg(src + j * 32);
+            }
+#pragma unroll
+            for (int q = 0; q < PF; ++q) {
+              if (c + q <= c_last) {
+#pragma unroll
+                for (int j = 0; j < HALF; ++j) acc[j] = __fadd_rn(acc[j], in[q][j]);
+              }
+            }
           } else {
+            const float *src = p.ws + (size_t)share_slot(c, tile_u0, p.units, p.sk_workers) * slot_floats + within;
 #pragma unroll
             for (int j = 0; j < HALF; ++j) acc[j] = __fadd_rn(acc[j], ptx::ld_cg_ordered(src + j * 32));
           }
@@ -816,8 +929,12 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
   void *ws = nullptr;
   if (rc == B200_OK && !(e->flags & B200_ENGINE_NO_STREAMK)) {
     // whole tiles per CTA would leave SMs idle: share out the k range instead (TilePieces)
+    // (Where two parts of each tile occupy most SMs, no tile is cut into more: 64 x 8192 x 4096, 64 tiles, in up to four
+    // parts 22 us, in two 18; 64 x 4096 x 4096, 32 tiles, 15.1 and 16.9.)
     int shares = workers, first = 0;
+    const int most = 3 * total_tiles >= max_workers ? (int)std::min<long long>(max_workers, 2 * total_tiles) : max_workers;
     if (total_tiles <= b200_engine::kSkCounters / 2 && streamk_pays(total_tiles, p.num_k, max_workers, &shares)) {
+      shares = std::min(shares, most);
       if (b200_get(e, 2LL * shares * ranks * GB_BM * bn * 4, &ws) == B200_OK) {
         p.streamk = 1;
         p.units = (int)(total_tiles * p.num_k);
@@ -847,6 +964,13 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
   for (void *s : {blk[0], blk[1], ws})
     if (s) b200_put(e, s, 0);
   return rc;
+}
+
+template <int NT>
+static void launch_skinny(b200_engine *e, const BlockOperand &w, const BlockOperand &x, const BlocksParams &p) {
+  auto kern = w.e5m2 ? (x.e5m2 ? gemm_blocks_skinny_kernel<NT, true, true> : gemm_blocks_skinny_kernel<NT, true, false>)
+                     : (x.e5m2 ? gemm_blocks_skinny_kernel<NT, false, true> : gemm_blocks_skinny_kernel<NT, false, false>);
+  launch_kernel(e, kern, (unsigned)((p.N + 15) / 16), 256, 0, w, x, p);
 }
 
 static BlockOperand block_operand(const void *data, int type, int block, bool k_contiguous, long long ld, const float *scales,
@@ -914,6 +1038,18 @@ int b200_gemm_blocks(b200_engine *e, int ctype, int transA, int transB, int64_t 
   if (K > 0) {
     const StoredOperand sa{(const uint8_t *)A, transA ? K : M, transA ? M : K, lda};
     const StoredOperand sb{(const uint8_t *)B, transB ? N : K, transB ? K : N, ldb};
+    // Few rows, k contiguous and 16-byte loads possible: the kernel for these, as long as B is not so large that the tensor
+    // cores' longer way is hidden behind its reading. us, this kernel / the other: 1 x 4096 x 4096 6.7 / 12.7, 8 x 8192 x 4096
+    // 11.9 / 16.2, 1 x 4096 x 16384 17.8 / 25.5, 8 x 16384 x 8192 38 / 29; two column tiles: 16 x 4096 x 4096 9.8 / 13.2,
+    // 16 x 8192 x 4096 18.3 / 16.6. Not where a result may not depend on the batch.
+    const long long most = M <= 8 ? 100LL << 20 : 16LL << 20;
+    if (M <= 16 && (long long)N * K <= most && !transA && transB && !(e->flags & B200_ENGINE_NO_STREAMK) &&
+        (((uintptr_t)A | (uintptr_t)B | (uintptr_t)lda | (uintptr_t)ldb | (uintptr_t)K) & 15) == 0) {
+      if (M <= 8) launch_skinny<1>(e, b, a, p);
+      else launch_skinny<2>(e, b, a, p);
+      B200_CHECK_LAUNCH(e, "gemm_blocks_skinny_kernel");
+      return B200_OK;
+    }
     rc = gemm_blocks_tc(e, sa, sb, a, b, transA != 0, transB == 0, p);
     if (rc != B200_ERR_OOM) return rc;
   }

@@ -108,6 +108,14 @@ class Tensor:
             self.ptr = None
 
 
+_NP_F32, _NP_F64, _NP_I64 = np.dtype(np.float32), np.dtype(np.float64), np.dtype(np.int64)
+
+
+def _fits(t, size, dtype):
+    """Whether an optional tensor holds `size` values of `dtype` (a call asks it for each of its tensors)."""
+    return t is None or (t.size == size and (t.dtype is dtype or t.dtype == dtype))
+
+
 _F8 = {"e4m3": _lib.E4M3, "e5m2": _lib.E5M2}
 _BLOCK = {"row": (_lib.BLOCK_ROW, 1, 128), "col": (_lib.BLOCK_COL, 128, 1), "tile": (_lib.BLOCK_TILE, 128, 128)}
 
@@ -128,6 +136,7 @@ class BlockTensor:
             raise B200Error(_lib.ERR_INVALID, f"BlockTensor: {block} blocks of a {q.shape} matrix have float32 scales of "
                                               f"shape {want}, not {scales.dtype} {scales.shape}")
         self.q, self.scales, self.format, self.block = q, scales, format, block
+        self.qtype, self.block_code = _F8[format], _BLOCK[block][0]
 
     @staticmethod
     def scale_shape(shape, block):
@@ -452,39 +461,43 @@ class Engine:
             raise B200Error(_lib.ERR_INVALID, f"QuantizeBlocks: {x.shape} does not fit {prealloc.shape}")
         rows, cols = x.shape
         dt = _lib.BF16 if getattr(x, "is_bf16", False) else dtype_code(x.dtype)
-        check(lib.b200_quantize_blocks(self.h, dt, _F8[prealloc.format], _BLOCK[prealloc.block][0], x.ptr, cols, rows,
-                                       cols, prealloc.q.ptr, cols, prealloc.scales.ptr), self.h)
+        check(lib.b200_quantize_blocks(self.h, dt, prealloc.qtype, prealloc.block_code, x.ptr, cols, rows, cols,
+                                       prealloc.q.ptr, cols, prealloc.scales.ptr), self.h)
         return prealloc
 
     def MatMulBlocks(self, a, b, prealloc, transA=False, transB=False, bias=None, bias_kind="col", act=None, alpha=0.0,
                      incr=False):
         """prealloc = op(a) @ op(b) of two BlockTensors, or prealloc += it with incr; prealloc is float32 or bf16, the
         bias float32. The blocks of both operands have to lie along k: see b200_gemm_blocks."""
-        (ar, ac), (br, bc) = a.shape, b.shape
+        q, r = a.q, b.q
+        (ar, ac), (br, bc) = q.shape, r.shape
         M, K = (ac, ar) if transA else (ar, ac)
         K2, N = (bc, br) if transB else (br, bc)
         if K != K2:
             raise B200Error(_lib.ERR_INVALID, f"MatMulBlocks: inner dimensions differ ({K} vs {K2})")
         if prealloc.size != M * N:
             raise B200Error(_lib.ERR_INVALID, "MatMulBlocks: prealloc has the wrong size")
-        if bias is not None and (bias.dtype != np.float32 or bias.size != (N if bias_kind == "col" else M)):
+        if bias is not None and not _fits(bias, N if bias_kind == "col" else M, _NP_F32):
             raise B200Error(_lib.ERR_INVALID, "MatMulBlocks: the bias does not match the result")
         ct = _lib.BF16 if getattr(prealloc, "is_bf16", False) else dtype_code(prealloc.dtype)
-        ep = _epilogue(bias, bias_kind, act, alpha, accumulate=incr)
-        check(lib.b200_gemm_blocks(self.h, ct, int(transA), int(transB), M, N, K,
-                                   a.q.ptr, _F8[a.format], _BLOCK[a.block][0], ac, a.scales.ptr,
-                                   b.q.ptr, _F8[b.format], _BLOCK[b.block][0], bc, b.scales.ptr,
-                                   prealloc.ptr, N, C.byref(ep) if ep else None), self.h)
+        ep = None
+        if bias is not None or act is not None or incr:
+            ep = C.byref(_epilogue(bias, bias_kind, act, alpha, accumulate=incr))
+        rc = lib.b200_gemm_blocks(self.h, ct, transA, transB, M, N, K, q.ptr, a.qtype, a.block_code, ac, a.scales.ptr,
+                                  r.ptr, b.qtype, b.block_code, bc, b.scales.ptr, prealloc.ptr, N, ep)
+        if rc:
+            check(rc, self.h)
         return prealloc
 
     # ---- log probabilities of given tokens ---------------------------------------------------------
     @staticmethod
-    def _stat_checks(who, x, rows, stats):
-        stat = np.float64 if x.dtype == np.float64 else np.float32
+    def _stat_error(who, stat, stats):
         for name, t, size in stats:
-            if t is not None and (t.size != size or t.dtype != stat):
-                raise B200Error(_lib.ERR_INVALID, f"{who}: {name} has to hold {size} values of {np.dtype(stat)}, not "
-                                                  f"{t.size} of {t.dtype}")
+            if not _fits(t, size, stat):
+                raise B200Error(_lib.ERR_INVALID, f"{who}: {name} has to hold {size} values of {stat}, not {t.size} of "
+                                                  f"{t.dtype}")
+        raise B200Error(_lib.ERR_INVALID, f"{who}: targets and alternatives are int64, one target and as many alternatives "
+                                          "for each row")
 
     def TokenLogProbs(self, x, targets, logp, entropy=None, lse=None, top_logp=None, top_index=None):
         """The log probabilities logp of the tokens `targets` (int64, -1 for none) under the logits x (rows, vocab) of
@@ -492,34 +505,38 @@ class Engine:
         top_index.shape[1] alternatives. What is None is left out: see b200_token_logprobs."""
         rows, vocab = x.shape
         top = 0 if top_index is None else top_index.size // max(rows, 1)
-        self._stat_checks("TokenLogProbs", x, rows, (("logp", logp, rows), ("entropy", entropy, rows), ("lse", lse, rows),
+        stat = _NP_F64 if x.dtype == _NP_F64 else _NP_F32
+        if not (_fits(logp, rows, stat) and _fits(entropy, rows, stat) and _fits(lse, rows, stat) and
+                _fits(top_logp, rows * top, stat) and _fits(targets, rows, _NP_I64) and
+                _fits(top_index, rows * top, _NP_I64)):
+            self._stat_error("TokenLogProbs", stat, (("logp", logp, rows), ("entropy", entropy, rows), ("lse", lse, rows),
                                                      ("top_logp", top_logp, rows * top)))
-        for t, size in ((targets, rows), (top_index, rows * top)):
-            if t is not None and (t.dtype != np.int64 or t.size != size):
-                raise B200Error(_lib.ERR_INVALID, "TokenLogProbs: tokens are int64, one target for each row and as many "
-                                                  "alternatives for each")
         dt = _lib.BF16 if getattr(x, "is_bf16", False) else dtype_code(x.dtype)
-        p = [None if t is None else t.ptr for t in (targets, logp, entropy, lse, top_logp, top_index)]
-        check(lib.b200_token_logprobs(self.h, dt, x.ptr, vocab, rows, vocab, p[0], p[1], p[2], p[3], top, p[4], p[5]),
-              self.h)
+        rc = lib.b200_token_logprobs(self.h, dt, x.ptr, vocab, rows, vocab, targets and targets.ptr, logp and logp.ptr,
+                                     entropy and entropy.ptr, lse and lse.ptr, top, top_logp and top_logp.ptr,
+                                     top_index and top_index.ptr)
+        if rc:
+            check(rc, self.h)
         return logp
 
     def TokenLogProbsDiff(self, x, targets, lse, entropy, grad_logp, prealloc, grad_entropy=None):
         """The gradient of sum(grad_logp * logp) + sum(grad_entropy * entropy) with respect to the logits x, from the
         lse and entropy that TokenLogProbs wrote; prealloc may be x: see b200_token_logprobs_bwd."""
         rows, vocab = x.shape
-        self._stat_checks("TokenLogProbsDiff", x, rows, (("lse", lse, rows), ("entropy", entropy, rows),
-                                                         ("grad_logp", grad_logp, rows),
-                                                         ("grad_entropy", grad_entropy, rows)))
-        if targets.dtype != np.int64 or targets.size != rows:
-            raise B200Error(_lib.ERR_INVALID, "TokenLogProbsDiff: targets are int64, one for each row")
+        stat = _NP_F64 if x.dtype == _NP_F64 else _NP_F32
+        if not (_fits(lse, rows, stat) and _fits(entropy, rows, stat) and _fits(grad_logp, rows, stat) and
+                _fits(grad_entropy, rows, stat) and _fits(targets, rows, _NP_I64)):
+            self._stat_error("TokenLogProbsDiff", stat, (("lse", lse, rows), ("entropy", entropy, rows),
+                                                         ("grad_logp", grad_logp, rows), ("grad_entropy", grad_entropy, rows)))
         bf = getattr(x, "is_bf16", False)
-        if prealloc.size != x.size or prealloc.dtype != x.dtype or getattr(prealloc, "is_bf16", False) != bf:
+        if prealloc is not x and (prealloc.size != x.size or prealloc.dtype != x.dtype or
+                                  getattr(prealloc, "is_bf16", False) != bf):
             raise B200Error(_lib.ERR_INVALID, "TokenLogProbsDiff: prealloc does not match the logits")
-        check(lib.b200_token_logprobs_bwd(self.h, _lib.BF16 if bf else dtype_code(x.dtype), x.ptr, vocab, rows, vocab,
-                                          targets.ptr, lse.ptr, None if entropy is None else entropy.ptr, grad_logp.ptr,
-                                          None if grad_entropy is None else grad_entropy.ptr, prealloc.ptr, vocab),
-              self.h)
+        rc = lib.b200_token_logprobs_bwd(self.h, _lib.BF16 if bf else dtype_code(x.dtype), x.ptr, vocab, rows, vocab,
+                                         targets and targets.ptr, lse and lse.ptr, entropy and entropy.ptr,
+                                         grad_logp and grad_logp.ptr, grad_entropy and grad_entropy.ptr, prealloc.ptr, vocab)
+        if rc:
+            check(rc, self.h)
         return prealloc
 
     # ---- softmax / reductions ---------------------------------------------------------------
