@@ -223,7 +223,7 @@ struct BlocksTcParams {
   void *C;
   long long c_row, c_col;       // elements between rows and columns; one of them is 1
   int c_bf16;
-  int c_vec, c_tma;             // rows can be stored 16 bytes at a time; the tile leaves by TMA stores
+  int c_tma;                    // the tile leaves by TMA stores
   int tiles_m, tiles_n, num_k, group_m;
   int stages, stage_bytes;
   // how the work is shared between the CTAs (TilePieces, tc_common.cuh)
@@ -668,7 +668,6 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
           }
         }
       } else {
-        const long long at = (long long)m * p.c_row + n0;
         if (HALF >= 32 && p.c_tma) {
           // A lane holds a row. The warp's part of the tile goes to shared memory, boxes of 32 rows of 128 bytes in the
           // 128-byte swizzle, and from there by TMA stores that drain while the next tile is multiplied: all SMs
@@ -714,42 +713,32 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
               send(c, 2);
             }
           }
-        } else if (m < p.M) {
-          if (p.c_bf16) {
-            __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(p.C) + at;
-            if (p.c_vec && valid == HALF) {
+        } else {
+          // Anything else (rows that do not start on 16-byte boundaries, results that are added) goes through shared
+          // memory too, 32 columns at a time, and leaves row by row: from the lanes' registers an instruction would
+          // touch 32 rows (1000 x 625 x 1152 float32: @LAYER@).
+          constexpr int W = HALF < 32 ? HALF : 32, PITCH = W + 1;
+          float *out = reinterpret_cast<float *>(stage_out + ew * GB_OUT);
 #pragma unroll
-              for (int j = 0; j < HALF; j += 8) {
-                uint4 w;
-                uint32_t *ww = reinterpret_cast<uint32_t *>(&w);
+          for (int c = 0; c < HALF; c += W) {
+            __syncwarp();
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                  const __nv_bfloat162 h = __floats2bfloat162_rn(acc[j + 2 * t], acc[j + 2 * t + 1]);
-                  ww[t] = *reinterpret_cast<const uint32_t *>(&h);
+            for (int j = 0; j < W; ++j) out[lane * PITCH + j] = acc[c + j];
+            __syncwarp();
+            const int j = lane % W, rows = min(32, p.M - mw);
+            if (c + j < valid) {
+              const long long first = (long long)mw * p.c_row + n0 + c + j;
+#pragma unroll 8
+              for (int r = lane / W; r < rows; r += 32 / W) {
+                const float v = out[r * PITCH + j];
+                const long long x = first + r * p.c_row;
+                if (p.c_bf16) {
+                  reinterpret_cast<__nv_bfloat16 *>(p.C)[x] = __float2bfloat16_rn(v);
+                } else {  // Incr mode: the rounded result is added to what C holds
+                  float *f = reinterpret_cast<float *>(p.C) + x;
+                  *f = p.ep.accumulate ? __fadd_rn(*f, v) : v;
                 }
-                *reinterpret_cast<uint4 *>(out + j) = w;
               }
-            } else {
-#pragma unroll
-              for (int j = 0; j < HALF; ++j)
-                if (j < valid) out[j] = __float2bfloat16_rn(acc[j]);
-            }
-          } else {
-            float *out = reinterpret_cast<float *>(p.C) + at;
-            if (p.c_vec && valid == HALF) {
-#pragma unroll
-              for (int j = 0; j < HALF; j += 4) {
-                float4 v = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-                if (p.ep.accumulate) {  // Incr mode: the rounded result is added to what C holds
-                  const float4 old = *reinterpret_cast<const float4 *>(out + j);
-                  v = make_float4(__fadd_rn(old.x, v.x), __fadd_rn(old.y, v.y), __fadd_rn(old.z, v.z), __fadd_rn(old.w, v.w));
-                }
-                *reinterpret_cast<float4 *>(out + j) = v;
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < HALF; ++j)
-                if (j < valid) out[j] = p.ep.accumulate ? __fadd_rn(out[j], acc[j]) : acc[j];
             }
           }
         }
@@ -800,7 +789,7 @@ __global__ void __launch_bounds__(256) repack_kernel(const RepackJob j0, const R
 template <int BN, bool PAIR = false>
 static int launch_blocks_tc(b200_engine *e, const CUtensorMap *tm, const BlocksTcParams &p, int grid) {
   auto kern = gemm_blocks_tc_kernel<BN, PAIR>;
-  const size_t smem = (size_t)p.stages * p.stage_bytes + (p.c_tma ? gb_epi_warps(BN) * GB_OUT : 0) + 1024;
+  const size_t smem = (size_t)p.stages * p.stage_bytes + (p.c_row != 1 ? gb_epi_warps(BN) * GB_OUT : 0) + 1024;
   static std::atomic<int> attr_dev_mask{0};
   if (!(attr_dev_mask & (1 << (e->device & 31)))) {
     cudaFuncAttributes fa;
@@ -870,7 +859,6 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
   p.c_row = swap ? 1 : q.ldc;
   p.c_col = swap ? q.ldc : 1;
   p.c_bf16 = q.c_bf16;
-  p.c_vec = !swap && (uintptr_t)q.C % 16 == 0 && q.ldc % (q.c_bf16 ? 8 : 4) == 0;
   p.ep = ep;
   p.err_flag = e->d_flags + 2;
   p.num_k = (int)((q.K + GB_BK - 1) / GB_BK);
@@ -879,7 +867,8 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
   int bn = 256;
   while (bn > 64 && (long long)p.tiles_m * ((N + bn - 1) / bn) < e->sm_count) bn /= 2;
   while (bn > 16 && bn / 2 >= N) bn /= 2;
-  p.c_tma = p.c_vec && !ep.accumulate && bn >= (q.c_bf16 ? 128 : 64);  // a warp's columns fill a box of 128 bytes
+  p.c_tma = !swap && (uintptr_t)q.C % 16 == 0 && q.ldc % (q.c_bf16 ? 8 : 4) == 0 && !ep.accumulate &&
+            bn >= (q.c_bf16 ? 128 : 64);  // a warp's columns fill a box of 128 bytes
   p.tiles_n = (int)((N + bn - 1) / bn);
   // the widest tiles are shared by pairs of CTAs
   const bool pair = !(e->flags & B200_ENGINE_NO_PAIRS) && bn == 256;
@@ -890,7 +879,7 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
     return set_error(e, B200_ERR_UNSUPPORTED, "b200_gemm_blocks: %lld output tiles are more than one launch takes", total_tiles);
   p.group_m = std::min(p.tiles_m, 8 / ranks);
   p.stage_bytes = GB_SLAB + (b_mn ? std::max(bn / ranks, 128) : bn / ranks) * 128;
-  const int budget = (int)std::min<size_t>(e->smem_optin, 227 * 1024) - 1024 - 14 * 1024 - (p.c_tma ? gb_epi_warps(bn) * GB_OUT : 0);  // static part, alignment
+  const int budget = (int)std::min<size_t>(e->smem_optin, 227 * 1024) - 1024 - 14 * 1024 - (p.c_row != 1 ? gb_epi_warps(bn) * GB_OUT : 0);  // static part, alignment
   p.stages = std::min(gb_max_stages(bn), budget / p.stage_bytes);
   p.idesc = make_idesc(0, a_mn, b_mn, GB_BM * ranks, bn) | ((uint32_t)a.e5m2 << 7) | ((uint32_t)b.e5m2 << 10);
 
