@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
         } else {
           // Anything else (rows that do not start on 16-byte boundaries, results that are added) goes through shared
           // memory too, 32 columns at a time, and leaves row by row: from the lanes' registers an instruction would
-          // touch 32 rows (1000 x 625 x 1152 float32: @LAYER@).
+          // touch 32 rows (1000 x 625 x 1152 float32 16.1 -> 13.2 us).
           constexpr int W = HALF < 32 ? HALF : 32, PITCH = W + 1;
           float *out = reinterpret_cast<float *>(stage_out + ew * GB_OUT);
 #pragma unroll
@@ -779,8 +779,19 @@ __global__ void __launch_bounds__(256) repack_kernel(const RepackJob j0, const R
       uint8_t b[16];
       uint4 v;
     } o;
+    if (c >= 4 && c + 20 <= j.cols) {
+      // five aligned words around the sixteen bytes, all of them inside the row (4095^3: 134 -> 126 us)
+      const uint32_t *w4 = reinterpret_cast<const uint32_t *>((uintptr_t)s & ~(uintptr_t)3);
+      const unsigned by = ((unsigned)(uintptr_t)s & 3u) * 8u;
+      uint32_t in[5];
 #pragma unroll
-    for (int t = 0; t < 16; ++t) o.b[t] = c + t < j.cols ? s[t] : 0;
+      for (int t = 0; t < 5; ++t) in[t] = t < 4 || by ? __ldg(w4 + t) : 0u;
+      o.v = make_uint4(__funnelshift_r(in[0], in[1], by), __funnelshift_r(in[1], in[2], by), __funnelshift_r(in[2], in[3], by),
+                       __funnelshift_r(in[3], in[4], by));
+    } else {
+#pragma unroll
+      for (int t = 0; t < 16; ++t) o.b[t] = c + t < j.cols ? s[t] : 0;
+    }
     *reinterpret_cast<uint4 *>(j.dst + r * j.ldo + c) = o.v;
   }
 }
@@ -863,15 +874,32 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
   p.err_flag = e->d_flags + 2;
   p.num_k = (int)((q.K + GB_BK - 1) / GB_BK);
   p.tiles_m = (int)((M + GB_BM - 1) / GB_BM);
-  // tile width: the widest that still gives every SM a tile
+  // Tile width. A k-block costs a CTA about as much on 64 columns as on 128 (four instructions and a commit take 514
+  // cycles to issue, whatever their width), a pair of CTAs on 256 x 256 one and a half times that: the width is the one
+  // whose rounds of tiles take least, the widest of equals. (The widest that gives every SM a tile, which
+  // bf16 products take, made 512 x 4096 x 4096 in two rounds of 64 columns, 32 us, and 1024 x 4096 x 4096 in two of 128, 34.)
+  const bool may_pair = !(e->flags & B200_ENGINE_NO_PAIRS), may_share = !(e->flags & B200_ENGINE_NO_STREAMK);
+  auto tiles_of = [&](int width) {
+    const long long rows = width == 256 && may_pair ? 256 : 128;
+    return (M + rows - 1) / rows * ((N + width - 1) / width);
+  };
+  auto cost = [&](int width) {  // us
+    const bool paired = width == 256 && may_pair;
+    const long long workers = paired ? e->sm_count / 2 : e->sm_count, tiles = tiles_of(width);
+    const double block = width == 256 ? 0.62 : (width == 128 ? 0.42 : 0.39);
+    const double whole = (double)((tiles + workers - 1) / workers) * p.num_k * block;
+    if (!may_share || tiles >= workers) return whole;
+    const long long shares = std::min(workers, (3 * tiles >= workers ? 2 : 4) * tiles);
+    return std::min(whole, (double)(tiles * p.num_k) / shares * block + 4.0);
+  };
   int bn = 256;
-  while (bn > 64 && (long long)p.tiles_m * ((N + bn - 1) / bn) < e->sm_count) bn /= 2;
+  for (int width : {128, 64})
+    if (cost(width) < cost(bn) || bn / 2 >= N) bn = width;
   while (bn > 16 && bn / 2 >= N) bn /= 2;
   p.c_tma = !swap && (uintptr_t)q.C % 16 == 0 && q.ldc % (q.c_bf16 ? 8 : 4) == 0 && !ep.accumulate &&
             bn >= (q.c_bf16 ? 128 : 64);  // a warp's columns fill a box of 128 bytes
   p.tiles_n = (int)((N + bn - 1) / bn);
-  // the widest tiles are shared by pairs of CTAs
-  const bool pair = !(e->flags & B200_ENGINE_NO_PAIRS) && bn == 256;
+  const bool pair = may_pair && bn == 256;  // the widest tiles are shared by pairs of CTAs
   if (pair) p.tiles_m = (p.tiles_m + 1) / 2;
   const int ranks = pair ? 2 : 1, max_workers = e->sm_count / ranks;
   const long long total_tiles = (long long)p.tiles_m * p.tiles_n;
@@ -916,7 +944,7 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
   int workers = (int)std::min<long long>(total_tiles, max_workers);
   p.sk_workers = workers;
   void *ws = nullptr;
-  if (rc == B200_OK && !(e->flags & B200_ENGINE_NO_STREAMK)) {
+  if (rc == B200_OK && may_share) {
     // whole tiles per CTA would leave SMs idle: share out the k range instead (TilePieces)
     // (Where two parts of each tile occupy most SMs, no tile is cut into more: 64 x 8192 x 4096, 64 tiles, in up to four
     // parts 22 us, in two 18; 64 x 4096 x 4096, 32 tiles, 15.1 and 16.9.)

@@ -58,6 +58,7 @@ def close(got, want, lim):
     assert (err <= lim).all(), ((err / lim).max(), err.max())
 
 
+@np.errstate(over="ignore")
 def compare(got, x, targets, top, dtype):
     want = bu.logprobs(x, targets, top)
     lse = np.where(np.isfinite(want["lse"]), want["lse"], 0.0)
