@@ -805,6 +805,9 @@ static int launch_blocks_tc(b200_engine *e, const CUtensorMap *tm, const BlocksT
   if (!(attr_dev_mask & (1 << (e->device & 31)))) {
     cudaFuncAttributes fa;
     B200_CHECK_CUDA(e, cudaFuncGetAttributes(&fa, kern));
+    // what the widest tiles' warpgroups ask for has to be there, or they would wait for it for good
+    if (BN == 256 && fa.numRegs * gb_threads(BN) < 128 * 40 + 256 * 232)
+      return set_error(e, B200_ERR_CUDA, "gemm_blocks_tc_kernel was built with %d registers per thread", fa.numRegs);
     const size_t optin = std::min<size_t>(e->smem_optin, 227 * 1024);
     B200_CHECK_CUDA(e, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(optin - fa.sharedSizeBytes)));
     attr_dev_mask |= 1 << (e->device & 31);

@@ -637,7 +637,7 @@ int b200_token_logprobs(b200_engine *e, int dtype, const void *x, int64_t ldx, i
   std::lock_guard<std::recursive_mutex> lk(e->mu);
   B200_REQUIRE(e, dtype == B200_F32 || dtype == B200_F64 || dtype == B200_BF16, "b200_token_logprobs: dtype %d not supported",
                dtype);
-  B200_REQUIRE(e, rows >= 0 && vocab >= 1 && rows < (1LL << 31) && vocab < (1LL << 31), "b200_token_logprobs: bad extent");
+  B200_REQUIRE(e, rows >= 0 && vocab >= 1 && rows < (1LL << 31) && vocab <= (1LL << 30), "b200_token_logprobs: bad extent");
   B200_REQUIRE(e, top >= 0 && top <= B200_TOP_MAX && top <= vocab, "b200_token_logprobs: %d alternatives of %lld (at most %d)",
                top, (long long)vocab, B200_TOP_MAX);
   B200_REQUIRE(e, ldx >= vocab, "b200_token_logprobs: leading dimension too small (%lld)", (long long)ldx);
@@ -667,7 +667,7 @@ int b200_token_logprobs_bwd(b200_engine *e, int dtype, const void *x, int64_t ld
   std::lock_guard<std::recursive_mutex> lk(e->mu);
   B200_REQUIRE(e, dtype == B200_F32 || dtype == B200_F64 || dtype == B200_BF16,
                "b200_token_logprobs_bwd: dtype %d not supported", dtype);
-  B200_REQUIRE(e, rows >= 0 && vocab >= 1 && rows < (1LL << 31) && vocab < (1LL << 31), "b200_token_logprobs_bwd: bad extent");
+  B200_REQUIRE(e, rows >= 0 && vocab >= 1 && rows < (1LL << 31) && vocab <= (1LL << 30), "b200_token_logprobs_bwd: bad extent");
   B200_REQUIRE(e, ldx >= vocab && lddx >= vocab, "b200_token_logprobs_bwd: leading dimension too small (%lld %lld)",
                (long long)ldx, (long long)lddx);
   if (rows == 0) return B200_OK;

@@ -457,8 +457,8 @@ int b200_gemm_blocks(b200_engine *e, int ctype, int transA, int transB, int64_t 
 /* ---- log probabilities of given tokens -----------------------------------------------------------
  * What a classifier's or language model's loss, and its sampling, read from the logits: in gorgonia a LogSoftMax
  * (op_softmax.go:99-128) that is written whole, ByIndices on it (op_by_indices.go:90-97), and more passes for the
- * rest. Here one pass over x (rows x vocab, leading dimension ldx; B200_F32, B200_F64 or B200_BF16) writes for each row,
- * in float64 for B200_F64 and in float32 otherwise:
+ * rest. Here one pass over x (rows x vocab, vocab at most 2^30, leading dimension ldx; B200_F32, B200_F64 or
+ * B200_BF16) writes for each row, in float64 for B200_F64 and in float32 otherwise:
  *   lse     the log of the sum of the exponentials of the row (may be NULL);
  *   logp    that of the row's target, x[targets[row]] - lse (NULL with targets == NULL); 0 for a row whose target is B200_NO_TOKEN;
  *   entropy lse - sum p x, p = exp(x - lse) (may be NULL);

@@ -182,6 +182,27 @@ def test_matmul_larger(fresh, M, N, K, layout):
     check(multiply(e, a, b, M, N, ta, tb, bf16), a, b, K, ta, tb, bf16)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 1, 16), (1, 17, 48), (3, 33, 128), (8, 200, 1040), (8, 16, 8192), (9, 40, 256), (12, 200, 512),
+                                   (16, 48, 144), (16, 4096, 1024), (11, 1000, 2064)])
+@pytest.mark.parametrize("av,bv", [(True, False), (True, True), (False, False)])
+@pytest.mark.parametrize("af,bf", [("e4m3", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e4m3"), ("e5m2", "e5m2")])
+def test_matmul_few_rows(fresh, M, N, K, av, bv, af, bf):
+    """The tokens of a few sequences: weights (out, in), k a multiple of 16, one and two column tiles; bias of either
+    kind, activation, both types of the result, addition to it."""
+    e = fresh
+    a, b = operands(M + N, M, N, K, False, True, av, bv, af, bf)
+    got = multiply(e, a, b, M, N, False, True)
+    check(got, a, b, K, False, True)
+    check(multiply(e, a, b, M, N, False, True, True), a, b, K, False, True, True)
+    want, size = bu.matmul(a, b, False, True)
+    for kind, n in (("col", N), ("row", M)):
+        bias = util.normal(20, n) * np.float32(np.abs(want).mean())
+        c = e.tensor(np.ones((M, N), np.float32))
+        e.MatMulBlocks(upload(e, a), upload(e, b), c, transB=True, bias=e.tensor(bias), bias_kind=kind, act="rectify", incr=True)
+        t = (got + (bias if kind == "col" else bias[:, None])).astype(np.float32)
+        assert_bits_equal(c.numpy(), np.float32(1) + np.where(t >= 0, t, np.float32(0)))
+
+
 @pytest.mark.parametrize("ta,tb", [(False, True), (False, False), (True, False)])
 @pytest.mark.parametrize("af,bf", [("e4m3", "e5m2"), ("e5m2", "e4m3"), ("e5m2", "e5m2")])
 def test_matmul_formats(fresh, af, bf, ta, tb):

@@ -355,7 +355,7 @@ def test_refusals(fresh):
         return lib.b200_token_logprobs_bwd(e.h, dt, xp, ld, rows, vocab, t, lse, ent, g, h, dx, lddx)
     assert fwd() == 0 and fwd(rows=0, xp=None) == 0 and bwd() == 0 and bwd(rows=0, xp=None) == 0
     assert fwd(t=None, lp=None) == 0 and fwd(lse=None, ent=None) == 0
-    for bad in (dict(dt=3), dict(dt=9), dict(rows=-1), dict(vocab=0), dict(ld=99), dict(xp=None), dict(t=None), dict(lp=None),
+    for bad in (dict(dt=3), dict(dt=9), dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 30) + 1, ld=1 << 31), dict(ld=99), dict(xp=None), dict(t=None), dict(lp=None),
                 dict(top=33, tl=s.ptr, ti=i.ptr), dict(top=-1), dict(top=5, vocab=4, tl=s.ptr, ti=i.ptr), dict(top=2), dict(top=2, tl=s.ptr),
                 dict(tl=s.ptr), dict(xp=x.ptr + 2), dict(t=i.ptr + 4), dict(lse=s.ptr + 2)):
         assert fwd(**bad) == _lib.ERR_INVALID, bad
