@@ -130,7 +130,8 @@ __device__ __forceinline__ void mma_16x8x32(float (&d)[4], uint32_t a0, uint32_t
 // instruction's operands belong to does not matter as long as both operands agree. 1 x 4096 x 4096: 6.7 us,
 // of which 2.6 are the reading of B at the copy rate and most of the rest the launch and one way to memory.
 template <int NT, bool W5, bool X5>
-__global__ void __launch_bounds__(256, 2) gemm_blocks_skinny_kernel(const BlockOperand w, const BlockOperand x, const BlocksParams p) {
+__global__ void __launch_bounds__(256, 2)
+    gemm_blocks_skinny_kernel(const BlockOperand w, const BlockOperand x, const BlocksParams p) {
   ptx::grid_begin();
   __shared__ float s_sum[8][16][NT * 8 + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -269,13 +270,19 @@ __device__ __forceinline__ void scale_fma_pair(float &a0, float &a1, uint32_t p0
       : "r"(p0), "r"(p1), "f"(row), "f"(c0), "f"(c1));
 }
 
-// Warps: 0 loads (TMA), 1 issues MMAs and owns tensor memory, 2 and 3 bring the scales of the k-blocks into shared
-// memory, the others (8, or 4 where a tile is 32 columns or fewer) take each k-block's accumulator to registers, scaled, and store the tile at its end. A ring stage and an
+// Persistent: a CTA takes tiles of 128 x BN, k-block by k-block. Warps: 0 loads (TMA), 1 issues MMAs and owns tensor
+// memory, 2 and 3 bring the scales of the k-blocks into shared memory, the others (8, or 4 where a tile is 32 columns or
+// fewer) take each k-block's accumulator to registers, scaled, and store the tile at its end. A ring stage and an
 // accumulator are one k-block each; there are at least as many stages as accumulators, so that one commit per
 // k-block, on the stage's "done" barrier, serves the loader and the epilogue: that barrier's next phase cannot
 // complete before the epilogue has let go of the accumulator that this one announced.
 // PAIR: two CTAs of a cluster share a tile of 256 x 256. Each loads its own 128 rows of A and half of B's, the even one
 // issues the MMAs for both (cta_group::2) and keeps their barriers, each scales and stores its own 128 rows.
+//
+// What bounds it: the epilogue. Scales that change from block to block keep the tensor core from accumulating over
+// k, so each 128 x 256 sums of a k-block are loaded from tensor memory and added once per 514 cycles of MMAs; on their own
+// the loads and additions take 270 cycles and the MMAs run at 4.27 PFLOP/s, together a k-block takes about 900, in which
+// tensor memory serves both. 8192^3 575 us (1.9 PFLOP/s) in short bursts, 650 under the power limit; without the additions 487.
 template <int BN, bool PAIR>
 __global__ void __launch_bounds__(gb_threads(BN), 1)
     gemm_blocks_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -910,7 +917,8 @@ static int gemm_blocks_tc(b200_engine *e, StoredOperand sa, StoredOperand sb, Bl
     return set_error(e, B200_ERR_UNSUPPORTED, "b200_gemm_blocks: %lld output tiles are more than one launch takes", total_tiles);
   p.group_m = std::min(p.tiles_m, 8 / ranks);
   p.stage_bytes = GB_SLAB + (b_mn ? std::max(bn / ranks, 128) : bn / ranks) * 128;
-  const int budget = (int)std::min<size_t>(e->smem_optin, 227 * 1024) - 1024 - 14 * 1024 - (p.c_row != 1 ? gb_epi_warps(bn) * GB_OUT : 0);  // static part, alignment
+  const int budget = (int)std::min<size_t>(e->smem_optin, 227 * 1024) - 1024 - 14 * 1024 -
+                     (p.c_row != 1 ? gb_epi_warps(bn) * GB_OUT : 0);  // alignment, static part, the stores' buffers
   p.stages = std::min(gb_max_stages(bn), budget / p.stage_bytes);
   p.idesc = make_idesc(0, a_mn, b_mn, GB_BM * ranks, bn) | ((uint32_t)a.e5m2 << 7) | ((uint32_t)b.e5m2 << 10);
 
