@@ -271,6 +271,22 @@ def test_matmul_empty_sum(fresh):
     assert_bits_equal(c.numpy(), np.broadcast_to(bias, (30, 40)).copy())
 
 
+def test_matrices_without_rows_or_columns(fresh):
+    """Through the tensors' own calls: nothing to round, nothing to multiply, or nothing to sum."""
+    e = fresh
+    none, wide = e.empty_blocks((0, 256)), e.empty_blocks((40, 256), "tile")
+    assert none.scales.shape == (0, 2)
+    e.QuantizeBlocks(e.empty((0, 256)), none)
+    e.QuantizeBlocks(e.tensor(np.ones((40, 256), np.float32)), wide)
+    e.MatMulBlocks(none, wide, e.empty((0, 40)), transB=True)
+    a, b = e.empty_blocks((30, 0)), e.empty_blocks((0, 40), "tile")
+    c = e.tensor(np.full((30, 40), 5.0, np.float32))
+    e.MatMulBlocks(a, b, c, incr=True)
+    assert np.all(c.numpy() == 5.0)
+    e.MatMulBlocks(a, b, c)
+    assert np.all(c.numpy() == 0.0)
+
+
 @pytest.mark.parametrize("M", [2, 150])
 def test_matmul_values_that_are_not_finite(fresh, M):
     """A NaN spoils its row (column) of the result and nothing else, from a value as from a scale; infinities of

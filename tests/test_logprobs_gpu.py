@@ -322,6 +322,13 @@ def test_tokens_outside_the_vocabulary(fresh, vocab):
     e.tape_destroy(tape)
 
 
+def test_no_rows(fresh):
+    e = fresh
+    x, t, s = e.empty((0, 50)), e.empty((0,), np.int64), e.empty((0,))
+    e.TokenLogProbs(x, t, s, s, s, e.empty((0, 4)), e.empty((0, 4), np.int64))
+    e.TokenLogProbsDiff(x, t, s, s, s, x, grad_entropy=s)
+
+
 @pytest.mark.parametrize("rows,vocab,top,dtype", [(2, 100000, 20, "bf16"), (300, 3000, 5, "f32"), (64, 10, 2, "f64")])
 def test_repeats_to_the_bit(fresh, rows, vocab, top, dtype):
     e = fresh
