@@ -2,7 +2,8 @@
 //
 // C[m, n] = act(sum over k-blocks of sa(m, kb) sb(n, kb) (sum over the block's k of a[m, k] b[n, k]) + bias): the
 // inner sum is of products of 8-bit values, which fp32 holds exactly; it is taken to fp32 registers once per
-// block of 128 and multiplied by the product of the two scales there.
+// block of 128 and multiplied by the product of the two scales there, or by one after the other where their product is out
+// of range (Scaling).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -11,6 +12,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include "engine.h"
 #include "epilogue.cuh"
@@ -41,6 +43,30 @@ struct BlocksParams {
 __device__ __forceinline__ float f8_to_float(uint8_t v, int e5m2) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, e5m2 ? __NV_E5M2 : __NV_E4M3)));
 }
+
+// Whether the product of two scales is a normal number, and can multiply a block's sum as it is. As one comparison: the magnitude's
+// bits less those of the least normal number, both doubled, so that what lies below wraps round.
+constexpr uint32_t RANGE = 254u << 24;
+__device__ __forceinline__ uint32_t away_from_range(float product) { return (__float_as_uint(product) << 1) - (1u << 24); }
+__device__ __forceinline__ bool in_range(float product) { return away_from_range(product) < RANGE; }
+
+// The product of two scales in a form that can be applied in any case. The sum `part` of a block is 0 or between 2^-32 and 2^39
+// (or no finite number). Of two scales whose product is out of range, the one that is farther out is brought nearer by
+// 2^64, which is exact, and the result is put back as it is added: a product above the range has a scale above 2^63 and the
+// other one is 1 or more, one below has a scale below 2^-63 and the other one is 2^23 at most, so nothing in between
+// leaves the range unless the result has by far. Which form is taken depends on the two scales alone.
+struct Scaling {
+  float first, second, last;  // 1, 1 and the product where that is in range
+  __device__ __forceinline__ Scaling(float a, float b) {
+    const float product = __fmul_rn(a, b);
+    const bool fine = in_range(product), above = fabsf(product) > 1.f, swap = (fabsf(a) > fabsf(b)) != above;
+    first = fine ? 1.f : (swap ? b : a) * (above ? 0x1p-64f : 0x1p64f);
+    second = fine ? 1.f : (swap ? a : b);
+    last = fine ? product : (above ? 0x1p64f : 0x1p-64f);
+  }
+  __device__ __forceinline__ float near(float part) const { return __fmul_rn(__fmul_rn(part, first), second); }
+  __device__ __forceinline__ float add(float acc, float part) const { return __fmaf_rn(near(part), last, acc); }
+};
 
 // Any layout, alignment and size: 64 x 64 outputs per CTA, 4 x 4 per thread, 32 k at a time through shared memory.
 constexpr int GB_T = 64, GB_K = 32;
@@ -82,13 +108,13 @@ __global__ void __launch_bounds__(256) gemm_blocks_simt_kernel(const BlockOperan
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const long long m = m0 + ty + 16 * j, n = n0 + tx + 16 * j;
-        ra[j] = m < p.M ? a.scales[(m >> a.shift) * a.ss_i + (k0 >> 7) * a.ss_k] : 0.f;
-        rb[j] = n < p.N ? b.scales[(n >> b.shift) * b.ss_i + (k0 >> 7) * b.ss_k] : 0.f;
+        ra[j] = m < p.M ? a.scales[(m >> a.shift) * a.ss_i + (k0 >> 7) * a.ss_k] : 1.f;
+        rb[j] = n < p.N ? b.scales[(n >> b.shift) * b.ss_i + (k0 >> 7) * b.ss_k] : 1.f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(part[i][j], ra[i] * rb[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) acc[i][j] = Scaling(ra[i], rb[j]).add(acc[i][j], part[i][j]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -153,8 +179,13 @@ __global__ void __launch_bounds__(256, 2)
   auto bytes = [&](int r, int k) -> uint4 {
     return k < K ? __ldg(reinterpret_cast<const uint4 *>(row[r] + k)) : make_uint4(0, 0, 0, 0);
   };
-  constexpr int AHEAD = 4;  // k-blocks of w in flight per warp: 2 KB each
+  // k-blocks of w in flight per warp, 2 KB each (with two column tiles four do not fit the registers: 16 x 4096 x 4096 in the
+  // loop of calls 8.0 us instead of 7.1)
+  constexpr int AHEAD = NT == 1 ? 4 : 3;
   float acc[NT][4];
+  // The k-blocks are added without asking whether a product of two scales is in range: how far the products go is
+  // kept, and a warp that has met one out of range begins again with care.
+  uint32_t most = 0;
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -183,7 +214,41 @@ __global__ void __launch_bounds__(256, 2)
           mma_16x8x32<W5, X5>(part, a0.z, a1.z, a0.w, a1.w, b.z, b.w);
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[j][c] = __fmaf_rn(part[c], __fmul_rn(sw[c >> 1], sx[c & 1]), acc[j][c]);
+        for (int c = 0; c < 4; ++c) {
+          const float product = __fmul_rn(sw[c >> 1], sx[c & 1]);
+          most = max(most, away_from_range(product));
+          acc[j][c] = __fmaf_rn(part[c], product, acc[j][c]);
+        }
+      }
+    }
+  }
+  if (__any_sync(0xffffffffu, most >= RANGE)) {
+    long long first = n0;
+    asm volatile("" : "+l"(first));  // addresses are worked out again: kept over the loop above they cost it registers
+    auto load = [&](const BlockOperand &o, long long i, int k) -> uint4 {
+      return k < K ? __ldg(reinterpret_cast<const uint4 *>(o.data + i * o.si + k)) : make_uint4(0, 0, 0, 0);
+    };
+    auto scale = [](const BlockOperand &o, long long i, int kb) { return __ldg(o.scales + (i >> o.shift) * o.ss_i + kb * o.ss_k); };
+    auto wrow = [&](int i) { return min(first + g + 8 * i, p.N - 1); };
+    auto xrow = [&](int i) { return min((long long)i, p.M - 1); };
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[j][c] = 0.f;
+    for (int kb = warp; kb < nk; kb += 8) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = kb * 128 + h * 64 + t * 16;
+          const uint4 a0 = load(w, wrow(0), k), a1 = load(w, wrow(1), k), b = load(x, xrow(j * 8 + g), k);
+          mma_16x8x32<W5, X5>(part, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+          mma_16x8x32<W5, X5>(part, a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          acc[j][c] = Scaling(scale(w, wrow(c >> 1), kb), scale(x, xrow(j * 8 + 2 * t + (c & 1)), kb)).add(acc[j][c], part[c]);
       }
     }
   }
@@ -278,12 +343,14 @@ __device__ __forceinline__ void scale_fma_pair(float &a0, float &a1, uint32_t p0
 // complete before the epilogue has let go of the accumulator that this one announced.
 // PAIR: two CTAs of a cluster share a tile of 256 x 256. Each loads its own 128 rows of A and half of B's, the even one
 // issues the MMAs for both (cta_group::2) and keeps their barriers, each scales and stores its own 128 rows.
+// COLS: a scale for each of the tile's columns, else one for each 128. (An argument of the template, not of the launch:
+// 4096 x 4096 x 8192 summed down columns 223 -> 210 us, the question after products out of range included.)
 //
 // What bounds it: the epilogue. Scales that change from block to block keep the tensor core from accumulating over
 // k, so each 128 x 256 sums of a k-block are loaded from tensor memory and added once per 514 cycles of MMAs; on their own
 // the loads and additions take 270 cycles and the MMAs run at 4.27 PFLOP/s, together a k-block takes about 900, in which
 // tensor memory serves both. 8192^3 575 us (1.9 PFLOP/s) in short bursts, 650 under the power limit; without the additions 487.
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool COLS>
 __global__ void __launch_bounds__(gb_threads(BN), 1)
     gemm_blocks_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                           const __grid_constant__ CUtensorMap tmC, const __grid_constant__ BlocksTcParams p) {
@@ -414,7 +481,7 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
     // Rows and columns beyond the matrix get a scale of the last one: they are not stored.
     if (warp >= 2) {
       const int t = threadIdx.x - 64;
-      const bool row_each = p.a_shift == 0, col_each = p.b_shift == 0;
+      const bool row_each = p.a_shift == 0;
       int slot = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -438,7 +505,7 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
             ptx::copy_async_4(to, a + (long long)(min(m0, p.M - 1) >> 7) * p.as_i);
           }
           to += GB_BM;
-          if (col_each) {
+          if (COLS) {
 #pragma unroll
             for (int i = 0; i < BN; i += 64)
               if (i + t < BN) ptx::copy_async_4(to + i + t, b + (long long)min(n0 + i + t, p.N - 1) * p.bs_i);
@@ -503,7 +570,19 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
     const uint32_t acc_empty0 = at_leader(&acc_empty[0]);
     int stage = 0, buf = 0, slot = 0;
     uint32_t phase = 0, slot_phase = 0, epi_phase = 0;
-    const bool per_col = p.b_shift == 0;
+    // Whether some product of a scale of the warp's rows and one of its columns is out of range: the rows' times the least and
+    // the greatest magnitude of the columns', zeros apart.
+    auto any_far = [&](float row, const float *cols) -> bool {
+      float least = 3.40282347e38f, most = 0.f;
+      for (int j = lane; j < (COLS ? HALF : 1); j += 32) {
+        const float c = fabsf(cols[j]);
+        if (c != 0.f) least = fminf(least, c);
+        most = fmaxf(most, c);
+      }
+      least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
+      most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+      return __any_sync(0xffffffffu, row != 0.f && most != 0.f && !(in_range(__fmul_rn(row, least)) && in_range(__fmul_rn(row, most))));
+    };
     bool ok = true;
     auto epi_sync = [&]() -> bool {
       __syncwarp();
@@ -518,7 +597,7 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
       int mb, nb;
       decode(tile, mb, nb);
       const int m = (mb * RANKS + (int)rank) * GB_BM + quarter * 32 + lane, n0 = nb * BN + ch0;
-      const int row_at = p.a_shift == 0 ? quarter * 32 + lane : 0, col_at = GB_BM + (per_col ? ch0 : ch0 >> 7);
+      const int row_at = p.a_shift == 0 ? quarter * 32 + lane : 0, col_at = GB_BM + (COLS ? ch0 : ch0 >> 7);
       float acc[HALF];
 #pragma unroll
       for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
@@ -548,28 +627,80 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
         }
         __syncwarp();
         ptx::tc_fence_after_sync();
-#pragma unroll
-        for (int c = 0; c < HALF; c += CH) {
-          load(c);
+        auto take = [&](bool last) {  // what was loaded is in registers; after the last piece the accumulator is free
           ptx::tmem_ld_wait();
-          if (c + CH == HALF) {
-            ptx::tc_fence_before_sync();  // all of it is in registers: the accumulator is free
+          if (last) {
+            ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
               if (PAIR) ptx::mbar_arrive_cluster_tmem(acc_empty0 + (uint32_t)buf * 8u);
               else ptx::mbar_arrive(&acc_empty[buf]);
             }
           }
-          if (per_col) {
-#pragma unroll
-            for (int j = 0; j < CH; j += 4) {
-              const float4 s = *reinterpret_cast<const float4 *>(cols + c + j);
-              scale_fma_pair(acc[c + j], acc[c + j + 1], r[j], r[j + 1], row, s.x, s.y);
-              scale_fma_pair(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], row, s.z, s.w);
-            }
+        };
+        load(0);
+        // Seldom: scales whose product is out of range, or may be. (Asked without a branch while the first piece is on its way:
+        // a k-block of the epilogue is one chain of waits, and 100 cycles in front of it are 9 % of 512 x 4096 x 4096.)
+        bool odd;
+        if constexpr (COLS) {
+          // every scale in [2^-63, 2^63), a column or more to a lane: then the product of any two is in range
+          auto away = [](float v) { return (__float_as_uint(v) << 1) - (64u << 24); };
+          uint32_t most = away(row);
+          if constexpr (HALF <= 32) {
+            most = max(most, away(cols[lane & (HALF - 1)]));
+          } else if constexpr (HALF == 64) {
+            const float2 v = *reinterpret_cast<const float2 *>(cols + 2 * lane);
+            most = max(most, max(away(v.x), away(v.y)));
           } else {
+            const float4 v = *reinterpret_cast<const float4 *>(cols + 4 * lane);
+            most = max(max(most, away(v.x)), max(away(v.y), max(away(v.z), away(v.w))));
+          }
+          odd = most >= (126u << 24);
+        } else {
+          odd = !in_range(both);
+        }
+        odd = __any_sync(0xffffffffu, odd);
+        take(CH == HALF);
+        if constexpr (COLS) {
+          auto add_block = [&](auto careful) {
 #pragma unroll
-            for (int j = 0; j < CH; j += 2) fma_pair(acc[c + j], acc[c + j + 1], r[j], r[j + 1], both, both);
+            for (int c = 0; c < HALF; c += CH) {
+              if (c > 0) {
+                load(c);
+                take(c + CH == HALF);
+              }
+              if constexpr (decltype(careful)::value) {
+#pragma unroll
+                for (int j = 0; j < CH; ++j) acc[c + j] = Scaling(row, cols[c + j]).add(acc[c + j], __uint_as_float(r[j]));
+              } else {
+#pragma unroll
+                for (int j = 0; j < CH; j += 4) {
+                  const float4 s = *reinterpret_cast<const float4 *>(cols + c + j);
+                  scale_fma_pair(acc[c + j], acc[c + j + 1], r[j], r[j + 1], row, s.x, s.y);
+                  scale_fma_pair(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], row, s.z, s.w);
+                }
+              }
+            }
+          };
+          if (__builtin_expect(odd, 0) && any_far(row, cols)) add_block(std::true_type());
+          else add_block(std::false_type());
+        } else {
+          // (two forms of the sums, as above, made the compiler move them about: 8192^3 615 us instead of 564)
+          float last = both;
+#pragma unroll
+          for (int c = 0; c < HALF; c += CH) {
+            if (c > 0) {
+              load(c);
+              take(c + CH == HALF);
+            }
+            if (__builtin_expect(odd, 0)) {
+              const Scaling by(s_scale[slot][row_at], s_scale[slot][col_at]);
+              last = by.last;
+#pragma unroll
+              for (int j = 0; j < CH; ++j) r[j] = __float_as_uint(by.near(__uint_as_float(r[j])));
+            }
+#pragma unroll
+            for (int j = 0; j < CH; j += 2) fma_pair(acc[c + j], acc[c + j + 1], r[j], r[j + 1], last, last);
           }
         }
         if (++buf == NBUF) buf = 0;
@@ -804,9 +935,9 @@ __global__ void __launch_bounds__(256) repack_kernel(const RepackJob j0, const R
 }
 
 // grid: CTAs; pairs launch as clusters of two.
-template <int BN, bool PAIR = false>
-static int launch_blocks_tc(b200_engine *e, const CUtensorMap *tm, const BlocksTcParams &p, int grid) {
-  auto kern = gemm_blocks_tc_kernel<BN, PAIR>;
+template <int BN, bool PAIR, bool COLS>
+static int launch_blocks_tc_as(b200_engine *e, const CUtensorMap *tm, const BlocksTcParams &p, int grid) {
+  auto kern = gemm_blocks_tc_kernel<BN, PAIR, COLS>;
   const size_t smem = (size_t)p.stages * p.stage_bytes + (p.c_row != 1 ? gb_epi_warps(BN) * GB_OUT : 0) + 1024;
   static std::atomic<int> attr_dev_mask{0};
   if (!(attr_dev_mask & (1 << (e->device & 31)))) {
@@ -841,6 +972,11 @@ static int launch_blocks_tc(b200_engine *e, const CUtensorMap *tm, const BlocksT
   B200_CHECK_LAUNCH(e, "gemm_blocks_tc_kernel");
   e->flags_dirty = true;
   return B200_OK;
+}
+
+template <int BN, bool PAIR = false>
+static int launch_blocks_tc(b200_engine *e, const CUtensorMap *tm, const BlocksTcParams &p, int grid) {
+  return p.b_shift == 0 ? launch_blocks_tc_as<BN, PAIR, true>(e, tm, p, grid) : launch_blocks_tc_as<BN, PAIR, false>(e, tm, p, grid);
 }
 
 // One operand in the form that the TMA unit reads: rows x cols bytes as stored, pitch a multiple of 16.

@@ -438,7 +438,8 @@ int b200_reduce_all_static(b200_engine *e, int dtype, int kind, const void *x, i
  *
  * b200_gemm_blocks: C = act(op(A) op(B) + bias), or C + that (epilogue.accumulate, C of B200_F32 only). op(A) is
  *   M x K, op(B) K x N, transX != 0 as in b200_gemm. The blocks of an operand must lie 128 along k: A is ROW or TILE,
- *   with transA COL or TILE; B is COL or TILE, with transB ROW or TILE. The scales are any float32 values.
+ *   with transA COL or TILE; B is COL or TILE, with transB ROW or TILE. The scales are any float32 values; their product may
+ *   leave float32's range where a block's sum times both does not.
  *   ctype, C's type: B200_F32 or B200_BF16. Products are summed in fp32 over a block of 128 k on the tensor cores; a block's
  *   sum times its two scales is added up in fp32 registers, and the epilogue is applied there: one rounding at the
  *   end. ep->bias is a float32 vector for either ctype. K = 0 is the empty sum. C may not overlap the operands.
