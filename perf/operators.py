@@ -3,7 +3,9 @@
 A case is one call of one operator: a tensor rounded to 8 bits with a scale for each block of 128, a product of two such
 tensors, the log probabilities of given tokens with the entropy and the best alternatives, or the gradient of
 these. Inputs are drawn on the GPU from a seed. `run` computes a case in its plain form, from elementary torch
-operations in 32 bits (64 for float64 tensors), or, where `own` is set, by the framework's calls.
+operations in 32 bits (64 for float64 tensors), or, where `own` is set, by the framework's calls. These run on the
+engine's stream, which nothing orders with torch's: a state's first run waits for its inputs, and whoever reads the
+outputs, or gives the state's memory back, waits for the device first.
 """
 import math
 
@@ -275,10 +277,12 @@ _engine = None
 
 
 def _handles(s):
-    """The engine's handles of a state's tensors, which a program makes once beside the tensors."""
+    """The engine's handles of a state's tensors, which a program makes once beside the tensors, and after them: what
+    torch's stream has still to write there, or to read from memory that came to the outputs, is waited for."""
     global _engine
     import numpy as np
     from gorgonia_b200 import BlockTensor, Engine, Tensor
+    torch.cuda.current_stream().synchronize()
     if _engine is None:
         _engine = Engine(arena_bytes=1 << 30)
     case = s["case"]
