@@ -96,27 +96,32 @@ int sync_stream_checked(b200_engine *e) {
     B200_CHECK_CUDA(e, cudaMemcpyAsync(e->h_flags + 2, e->d_flags + 2, 3 * sizeof(int), cudaMemcpyDeviceToHost,
                                        e->stream));
     B200_CHECK_CUDA(e, cudaStreamSynchronize(e->stream));
+    // One error to a call: what else was found stays dirty, and raised on the device, for the next one that waits.
     e->flags_dirty = false;
-    const bool gather = e->gather_dirty, tokens = e->tokens_dirty && e->h_flags[4] != 0;
-    e->gather_dirty = false;
-    e->tokens_dirty = false;
-    if (tokens) cudaMemsetAsync(e->d_flags + 4, 0, sizeof(int), e->stream);
     if (e->h_flags[2] != 0) {
       e->h_flags[2] = 0;
       cudaMemsetAsync(e->d_flags + 2, 0, sizeof(int), e->stream);
       // a kernel that gave up may have left tiles half delivered: re-arm the arrival counters
       cudaMemsetAsync(e->sk_counters, 0, b200_engine::kSkCounters * sizeof(int), e->stream);
       cudaMemsetAsync(e->f16_recs, 0, 256, e->stream);
+      e->flags_dirty = e->gather_dirty || e->tokens_dirty;
       return set_error(e, B200_ERR_TIMEOUT, "a device-side wait ran out of time; results of the last "
                        "kernels are incomplete");
     }
-    if (gather && e->h_flags[3] != 0) {
+    const bool gather = e->gather_dirty && e->h_flags[3] != 0;
+    e->gather_dirty = false;
+    if (gather) {
       cudaMemsetAsync(e->d_flags + 3, 0, sizeof(int), e->stream);
-      return set_error(e, B200_ERR_INVALID, "a replayed tape holds a gather whose index lies outside its "
-                       "range; those rows were not written");
+      e->flags_dirty = e->tokens_dirty;
+      return set_error(e, B200_ERR_INVALID, "a gather's index (in a replayed tape, or in a call that reported "
+                       "another error) lies outside its range; those rows were not written");
     }
-    if (tokens)
+    const bool tokens = e->tokens_dirty && e->h_flags[4] != 0;
+    e->tokens_dirty = false;
+    if (tokens) {
+      cudaMemsetAsync(e->d_flags + 4, 0, sizeof(int), e->stream);
       return set_error(e, B200_ERR_INVALID, "a target of b200_token_logprobs lies outside the vocabulary");
+    }
     return B200_OK;
   }
   B200_CHECK_CUDA(e, cudaStreamSynchronize(e->stream));

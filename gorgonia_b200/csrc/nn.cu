@@ -1705,7 +1705,10 @@ int b200_gather_axis(b200_engine *e, const void *x, const int64_t *idx, void *y,
   }
   B200_CHECK_CUDA(e, cudaMemcpyAsync(e->h_flags + 3, bad, sizeof(int), cudaMemcpyDeviceToHost, e->stream));
   rc = sync_stream_checked(e);
-  if (rc != B200_OK) return rc;
+  if (rc != B200_OK) {
+    if (e->h_flags[3]) e->gather_dirty = e->flags_dirty = true;  // for the next call that waits
+    return rc;
+  }
   if (e->h_flags[3])
     return set_error(e, B200_ERR_INVALID, "b200_gather_axis: an index lies outside [0, %lld)", (long long)n_rows);
   return B200_OK;
