@@ -324,20 +324,27 @@ template <typename T>
 static int launch_quantize(b200_engine *e, int qtype, int block, const T *x, long long ldx, long long rows, long long cols,
                            uint8_t *q, long long ldq, float *scales) {
   constexpr int V = 16 / sizeof(T);
-  if (block != B200_BLOCK_ROW && (rows + 127) / 128 > 65535)
-    return set_error(e, B200_ERR_UNSUPPORTED, "b200_quantize_blocks: %lld rows are more than one launch takes", rows);
   if ((cols + 31) / 32 >= (1LL << 31))
     return set_error(e, B200_ERR_UNSUPPORTED, "b200_quantize_blocks: %lld columns are more than one launch takes", cols);
   // 16-byte loads where every row's vectors lie on their boundaries, and what is stored for them too
   const bool vec = (uintptr_t)x % 16 == 0 && ldx % V == 0 && (uintptr_t)q % V == 0 && ldq % V == 0 && cols % V == 0;
-  if (qtype == B200_E5M2) {
-    if (vec) launch_quantize_as<T, V, true>(e, block, x, ldx, rows, cols, q, ldq, scales);
-    else launch_quantize_as<T, 1, true>(e, block, x, ldx, rows, cols, q, ldq, scales);
-  } else {
-    if (vec) launch_quantize_as<T, V, false>(e, block, x, ldx, rows, cols, q, ldq, scales);
-    else launch_quantize_as<T, 1, false>(e, block, x, ldx, rows, cols, q, ldq, scales);
+  auto launch = [&](const T *xr, long long n, uint8_t *qr, float *sr) {
+    if (qtype == B200_E5M2) {
+      if (vec) launch_quantize_as<T, V, true>(e, block, xr, ldx, n, cols, qr, ldq, sr);
+      else launch_quantize_as<T, 1, true>(e, block, xr, ldx, n, cols, qr, ldq, sr);
+    } else {
+      if (vec) launch_quantize_as<T, V, false>(e, block, xr, ldx, n, cols, qr, ldq, sr);
+      else launch_quantize_as<T, 1, false>(e, block, xr, ldx, n, cols, qr, ldq, sr);
+    }
+  };
+  // Tiles and columns have a block of the grid for each 128 rows, 65535 at most: more rows take several launches. (Rows that
+  // follow each other by ldx, a multiple of V where `vec` holds, keep their alignment.)
+  const long long piece = block == B200_BLOCK_ROW ? rows : 65535LL * 128;
+  const long long scales_of_128 = block == B200_BLOCK_COL ? cols : (cols + 127) / 128;
+  for (long long r = 0; r < rows; r += piece) {
+    launch(x + r * ldx, std::min(piece, rows - r), q + r * ldq, scales + r / 128 * scales_of_128);
+    B200_CHECK_LAUNCH(e, "quantize_kernel");
   }
-  B200_CHECK_LAUNCH(e, "quantize_kernel");
   return B200_OK;
 }
 
