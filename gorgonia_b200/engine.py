@@ -491,6 +491,12 @@ class Engine:
 
     # ---- log probabilities of given tokens ---------------------------------------------------------
     @staticmethod
+    def _matrix(x, who):
+        if len(x.shape) != 2:
+            raise B200Error(_lib.ERR_INVALID, f"{who}: the logits are a matrix (rows, vocab), not {x.shape}")
+        return x.shape
+
+    @staticmethod
     def _stat_error(who, stat, stats):
         for name, t, size in stats:
             if not _fits(t, size, stat):
@@ -503,7 +509,7 @@ class Engine:
         """The log probabilities logp of the tokens `targets` (int64, -1 for none) under the logits x (rows, vocab) of
         float32, float64 or bf16; the rows' entropy; the log of their sums of exponentials; and the best
         top_index.shape[1] alternatives. What is None is left out: see b200_token_logprobs."""
-        rows, vocab = x.shape
+        rows, vocab = self._matrix(x, "TokenLogProbs")
         top = 0 if top_index is None else top_index.size // max(rows, 1)
         stat = _NP_F64 if x.dtype == _NP_F64 else _NP_F32
         if not (_fits(logp, rows, stat) and _fits(entropy, rows, stat) and _fits(lse, rows, stat) and
@@ -522,7 +528,7 @@ class Engine:
     def TokenLogProbsDiff(self, x, targets, lse, entropy, grad_logp, prealloc, grad_entropy=None):
         """The gradient of sum(grad_logp * logp) + sum(grad_entropy * entropy) with respect to the logits x, from the
         lse and entropy that TokenLogProbs wrote; prealloc may be x: see b200_token_logprobs_bwd."""
-        rows, vocab = x.shape
+        rows, vocab = self._matrix(x, "TokenLogProbsDiff")
         stat = _NP_F64 if x.dtype == _NP_F64 else _NP_F32
         if not (_fits(lse, rows, stat) and _fits(entropy, rows, stat) and _fits(grad_logp, rows, stat) and
                 _fits(grad_entropy, rows, stat) and _fits(targets, rows, _NP_I64)):
