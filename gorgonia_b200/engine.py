@@ -125,10 +125,7 @@ class BlockTensor:
     blocks are 1 x 128, "col" 128 x 1, "tile" 128 x 128. A value stands for itself times its block's scale."""
 
     def __init__(self, q, scales, format="e4m3", block="row"):
-        if format not in _F8:
-            raise B200Error(_lib.ERR_INVALID, f"BlockTensor: format {format!r} is not one of {sorted(_F8)}")
-        if block not in _BLOCK:
-            raise B200Error(_lib.ERR_INVALID, f"BlockTensor: block {block!r} is not one of {sorted(_BLOCK)}")
+        self._check_kinds(block, format)
         if len(q.shape) != 2 or q.dtype != np.uint8:
             raise B200Error(_lib.ERR_INVALID, f"BlockTensor: values are a matrix of uint8, not {q.dtype} {q.shape}")
         want = self.scale_shape(q.shape, block)
@@ -137,6 +134,13 @@ class BlockTensor:
                                               f"shape {want}, not {scales.dtype} {scales.shape}")
         self.q, self.scales, self.format, self.block = q, scales, format, block
         self.qtype, self.block_code = _F8[format], _BLOCK[block][0]
+
+    @staticmethod
+    def _check_kinds(block, format):
+        if format not in _F8:
+            raise B200Error(_lib.ERR_INVALID, f"BlockTensor: format {format!r} is not one of {sorted(_F8)}")
+        if block not in _BLOCK:
+            raise B200Error(_lib.ERR_INVALID, f"BlockTensor: block {block!r} is not one of {sorted(_BLOCK)}")
 
     @staticmethod
     def scale_shape(shape, block):
@@ -452,8 +456,17 @@ class Engine:
 
     # ---- 8-bit matrices with a scale for each block of 128 ---------------------------------------
     def empty_blocks(self, shape, block="row", format="e4m3"):
+        BlockTensor._check_kinds(block, format)
+        shape = (shape,) if isinstance(shape, int) else tuple(shape)
+        if len(shape) != 2 or min(shape) < 0:
+            raise B200Error(_lib.ERR_INVALID, f"empty_blocks: a matrix has two dimensions, not {shape}")
         q = self.empty(shape, np.uint8)
-        return BlockTensor(q, self.empty(BlockTensor.scale_shape(shape, block), np.float32), format, block)
+        try:
+            scales = self.empty(BlockTensor.scale_shape(shape, block), np.float32)
+        except B200Error:
+            q.free()
+            raise
+        return BlockTensor(q, scales, format, block)
 
     def QuantizeBlocks(self, x, prealloc):
         """Rounds x (a float32 or bf16 matrix) to prealloc, a BlockTensor: see b200_quantize_blocks."""
