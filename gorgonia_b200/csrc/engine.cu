@@ -111,6 +111,7 @@ int sync_stream_checked(b200_engine *e) {
     const bool gather = e->gather_dirty && e->h_flags[3] != 0;
     e->gather_dirty = false;
     if (gather) {
+      e->h_flags[3] = 0;
       cudaMemsetAsync(e->d_flags + 3, 0, sizeof(int), e->stream);
       e->flags_dirty = e->tokens_dirty;
       return set_error(e, B200_ERR_INVALID, "a gather's index (in a replayed tape, or in a call that reported "

@@ -1681,8 +1681,7 @@ int b200_gather_axis(b200_engine *e, const void *x, const int64_t *idx, void *y,
   DeviceGuard g(e);
   int rc = flush_pending(e);
   if (rc != B200_OK) return rc;
-  int *bad = e->d_flags + 3;
-  B200_CHECK_CUDA(e, cudaMemsetAsync(bad, 0, sizeof(int), e->stream));
+  int *bad = e->d_flags + 3;  // raised by this or an earlier gather until it has been reported
   const bool w16 = row_bytes % 16 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)y % 16 == 0;
   const bool w4 = row_bytes % 4 == 0 && (uintptr_t)x % 4 == 0 && (uintptr_t)y % 4 == 0;
   if (w16) {
@@ -1709,8 +1708,11 @@ int b200_gather_axis(b200_engine *e, const void *x, const int64_t *idx, void *y,
     if (e->h_flags[3]) e->gather_dirty = e->flags_dirty = true;  // for the next call that waits
     return rc;
   }
-  if (e->h_flags[3])
+  if (e->h_flags[3]) {
+    e->h_flags[3] = 0;
+    cudaMemsetAsync(bad, 0, sizeof(int), e->stream);
     return set_error(e, B200_ERR_INVALID, "b200_gather_axis: an index lies outside [0, %lld)", (long long)n_rows);
+  }
   return B200_OK;
 }
 
