@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(256) gemm_blocks_simt_kernel(const BlockOperan
 // ------------------------------------------------------------------------------------------
 
 // D += A B for 16 x 8 x 32 8-bit values, in fp32. (tcgen05 has no business here: a tile's way through shared and tensor
-// memory costs more than the reading of B itself. 1 x 4096 x 4096 there: 12.4 us.)
+// memory costs more than the reading of B itself. 1 x 4096 x 4096 there: 11.5 us.)
 template <bool A5, bool B5>
 __device__ __forceinline__ void mma_16x8x32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                             uint32_t b1) {
@@ -153,8 +153,8 @@ __device__ __forceinline__ void mma_16x8x32(float (&d)[4], uint32_t a0, uint32_t
 
 // A block takes 16 rows of the weights w and all of x; its eight warps share the k-blocks, and their sums are added in the
 // order of the warps. In a warp, lane 4 g + t holds the 16 bytes from 16 t on of every 64 of rows g and g + 8: which k an
-// instruction's operands belong to does not matter as long as both operands agree. 1 x 4096 x 4096: 6.7 us,
-// of which 2.6 are the reading of B at the copy rate and most of the rest the launch and one way to memory.
+// instruction's operands belong to does not matter as long as both operands agree. 1 x 4096 x 4096: 5.4 us in a row of calls,
+// which is the host's call; reading B takes 2.6 at the copy rate.
 template <int NT, bool W5, bool X5>
 __global__ void __launch_bounds__(256, 2)
     gemm_blocks_skinny_kernel(const BlockOperand w, const BlockOperand x, const BlocksParams p) {
@@ -346,10 +346,12 @@ __device__ __forceinline__ void scale_fma_pair(float &a0, float &a1, uint32_t p0
 // COLS: a scale for each of the tile's columns, else one for each 128. (An argument of the template, not of the launch:
 // 4096 x 4096 x 8192 summed down columns 223 -> 210 us, the question after products out of range included.)
 //
-// What bounds it: the epilogue. Scales that change from block to block keep the tensor core from accumulating over
-// k, so each 128 x 256 sums of a k-block are loaded from tensor memory and added once per 514 cycles of MMAs; on their own
-// the loads and additions take 270 cycles and the MMAs run at 4.27 PFLOP/s, together a k-block takes about 900, in which
-// tensor memory serves both. 8192^3 575 us (1.9 PFLOP/s) in short bursts, 650 under the power limit; without the additions 487.
+// What bounds it: the epilogue's way from one k-block to the next. Scales that change from block to block keep the tensor core
+// from accumulating over k, so each 128 x 256 sums of a k-block are loaded from tensor memory and added once per 514 cycles
+// of MMAs (4.27 PFLOP/s on their own). 8192^3 takes 555 us (2.0 PFLOP/s) in short bursts, 640 under the power limit: 0.63 us a k-block,
+// some 1,200 cycles. Loads and additions on their own are 270 of them; without the additions the product takes 456 us,
+// without the wait for the scales, which are long there, 499. So the k-block is a chain of waits (scales, MMAs, two loads, the
+// arrival at the pair's even CTA), of which the parts that were measured do not make up the whole.
 template <int BN, bool PAIR, bool COLS>
 __global__ void __launch_bounds__(gb_threads(BN), 1)
     gemm_blocks_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -602,7 +604,7 @@ __global__ void __launch_bounds__(gb_threads(BN), 1)
 #pragma unroll
       for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
       // An accumulator is taken in pieces of CH columns: the fewer waits for tensor memory, the better (8192^3 with
-      // 16 columns a piece, the next one on its way: 613 us, with 32: 575, with 64 and nothing ahead: 562).
+      // 32 columns a piece 587 us, with 64 551).
       uint32_t r[CH];
       auto load = [&](int c) {
         const uint32_t at = lane_addr + (uint32_t)(buf * BN + c);
@@ -1203,9 +1205,10 @@ int b200_gemm_blocks(b200_engine *e, int ctype, int transA, int transB, int64_t 
     const StoredOperand sa{(const uint8_t *)A, transA ? K : M, transA ? M : K, lda};
     const StoredOperand sb{(const uint8_t *)B, transB ? N : K, transB ? K : N, ldb};
     // Few rows, k contiguous and 16-byte loads possible: the kernel for these, as long as B is not so large that the tensor
-    // cores' longer way is hidden behind its reading. us, this kernel / the other: 1 x 4096 x 4096 6.7 / 12.7, 8 x 8192 x 4096
-    // 11.9 / 16.2, 1 x 4096 x 16384 17.8 / 25.5, 8 x 16384 x 8192 38 / 29; two column tiles: 16 x 4096 x 4096 9.8 / 13.2,
-    // 16 x 8192 x 4096 18.3 / 16.6. Not where a result may not depend on the batch.
+    // cores' longer way is hidden behind its reading. us in a row of calls, this kernel / the other: 1 x 4096 x 4096 5.4 / 11.5,
+    // 8 x 8192 x 4096 8.7 / 14.8, 1 x 4096 x 16384 13.7 / 21.6, 8 x 16384 x 8192 34.8 / 28.9; two column tiles: 16 x 4096 x 4096 7.1 / 11.8,
+    // 16 x 8192 x 4096 12.7 / 14.9 (the line lies where the kernel's former loop lost, 18.3 / 16.6, and is kept: results on
+    // either side of it differ in their last bits). Not where a result may not depend on the batch.
     const long long most = M <= 8 ? 100LL << 20 : 16LL << 20;
     if (M <= 16 && (long long)N * K <= most && !transA && transB && !(e->flags & B200_ENGINE_NO_STREAMK) &&
         (((uintptr_t)A | (uintptr_t)B | (uintptr_t)lda | (uintptr_t)ldb | (uintptr_t)K) & 15) == 0) {

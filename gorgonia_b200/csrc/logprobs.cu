@@ -18,8 +18,10 @@
 // list: then only what lies above the bound is taken, and the first equals from the row's start on. What overflows
 // all the same (the best logits side by side in one share), and rows with a NaN, are searched once per alternative.
 //
-// Measured: 4096 x 32000 float32 86 us (94 % of the copy rate), with 5 alternatives 101, bf16 54 and 67; 8 x 131072
-// bf16 with 20 alternatives 10.7 us, without any 5.4; gradient of 4096 x 32000 bf16 81 us (99 % of the copy rate).
+// Measured: 4096 x 32000 float32 85 us (94 % of the copy rate), with 5 alternatives 100; 8 x 131072 bf16 with 20 alternatives
+// 10.5 us, without any 4.7; gradient of 4096 x 32000 bf16 81 us (99 % of the copy rate), float32 153. Not bound by HBM: bf16, 54 and 67
+// us (75 and 60 %: 74 % of the issue slots with 20 alternatives), and float64, 4096 x 16000 211 and 221 us (38 %), its
+// gradient 231 (70 %): the exponentials of 64 bits. Rows of a few classes have a warp each: 2^20 x 10 float32 608 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 

@@ -259,8 +259,9 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 // ---- CTA pairs: a cluster of two CTAs on neighbouring SMs driving one tcgen05.mma (cta_group::2) --
 // The even CTA of the pair (cluster rank 0) issues the instructions; they read A from each CTA's
 // own shared memory (128 rows each, M = 256), the first half of B's rows from rank 0 and the second
-// half from rank 1, and leave each CTA's 128 rows of D in that CTA's tensor memory. Nothing below is
-// a multicast: every load writes the issuing CTA's own shared memory, and a commit names one barrier.
+// half from rank 1, and leave each CTA's 128 rows of D in that CTA's tensor memory. No load below is
+// a multicast: each writes the issuing CTA's own shared memory. A commit names one barrier, but for that of kblock_f8,
+// which arrives on the barrier of both CTAs.
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));

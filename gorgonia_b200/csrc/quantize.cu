@@ -7,10 +7,10 @@
 // the conversion to 8 bits is the only rounding.
 //
 // One pass: a block's values stay in registers between the search for its largest and the rounding. Float32 is bound
-// by HBM (8192 x 4096 to e4m3 by rows 33 us, by columns or tiles 29: 78 and 89 % of the copy rate); bfloat16, half the
-// bytes for as many values, by tiles too (17.4 us, 89 %), by rows (20.3) and columns (23.8) by the instructions of
-// the blocks' maxima, of which a block of one row or column has as many as a tile for a 128th of the values. Rows that do
-// not start on 16-byte boundaries are read value by value (8191 x 4095 bf16 by rows 35 us).
+// by HBM (8192 x 4096 to e4m3 by rows 33 us, by columns or tiles 29: 78 and 89 % of the copy rate), and so is bfloat16 by tiles
+// (17.4 us, 89 %). By rows (20.3) and columns (23.8) bfloat16 is at no unit's limit: by rows 60 % of the issue slots, 39 % of the
+// DRAM rate and 42 % of the warps are in use (by columns it has not been looked at), so there are too few loads in flight.
+// Rows that do not start on 16-byte boundaries are read value by value (8191 x 4095 bf16 by rows 35 us).
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -469,7 +469,8 @@ int b200_gemm_blocks(b200_engine *e, int ctype, int transA, int transB, int64_t 
  * A logit of -Inf is a token that cannot be: its probability is 0 and it adds nothing to the entropy. A row of nothing
  * else has lse and log probabilities of -Inf and entropy 0; a row with a NaN or +Inf has NaN in their places.
  * A target outside [0, vocab) other than B200_NO_TOKEN: logp is NaN, and the next call that waits for the stream
- * (b200_sync, b200_memcpy_d2h, ...) returns B200_ERR_INVALID, also after the replay of a tape.
+ * (b200_sync, b200_memcpy_d2h, ...) returns B200_ERR_INVALID, also after the replay of a tape. (Such a call reports one
+ * error: where a wait has run out or a gather's index was bad too, those come first and the token with the call after.)
  *
  * b200_token_logprobs_bwd: the gradient with respect to the logits of sum grad_logp * logp + sum grad_entropy * entropy,
  *   dx[v] = grad_logp (delta(v = target) - p[v]) - grad_entropy p[v] (ln p[v] + entropy), from the lse and entropy that the
@@ -477,8 +478,8 @@ int b200_gemm_blocks(b200_engine *e, int ctype, int transA, int transB, int64_t 
  *   entropy is not read). The alternatives carry no gradient. dx (leading dimension lddx) has x's type and may be x
  *   itself. A row of nothing but -Inf gets zeros. A row without any gradient (no token or grad_logp 0, and grad_entropy
  *   0 or NULL) gets zeros whatever it holds; its lse and x need not be valid. p = exp(x - lse) with lse as its type
- *   holds it: logits beyond 10^5 in float32, a row masked with the type's lowest value throughout among them, lose
- *   digits there. */
+ *   holds it: logits beyond 10^5 in float32 lose digits there, and in a row masked with the type's lowest value throughout, whose
+ *   lse is that value, p is 1 for each token (mask with -Inf, or give such a row no token). */
 #define B200_NO_TOKEN ((int64_t)-1)
 #define B200_TOP_MAX 32
 int b200_token_logprobs(b200_engine *e, int dtype, const void *x, int64_t ldx, int64_t rows, int64_t vocab,
